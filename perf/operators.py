@@ -130,10 +130,11 @@ def _stored(x, fmt):
     x = x.float()
     top = x.abs().amax(dim=-1)
     live = top >= TINY
-    inv = torch.where(live, TOP[fmt] / top, torch.zeros_like(top))
+    # a code next to a border goes by the last bit of the factor: both quotients are rounded correctly
+    inv = torch.where(live, (TOP[fmt] / top.double()).float(), torch.zeros_like(top))
     scaled = x * inv[..., None]
     codes = scaled.round().to(torch.int8) if fmt == "int8" else scaled.to(torch.float8_e4m3fn)
-    return codes, torch.where(live, top / TOP[fmt], torch.zeros_like(top))
+    return codes, torch.where(live, (top.double() / TOP[fmt]).float(), torch.zeros_like(top))
 
 
 def _values(codes, scales):
