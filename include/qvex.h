@@ -586,6 +586,91 @@ int qvex_attention_decode(const uint16_t* proj, long p_stride, const uint16_t* q
 int qvex_rope_table(int rot_dim, float theta, int rows, float* table, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Paged KV cache, in bf16 or quantized to 8 bits as it is written: a pool of
+ * pages shared by sequences (and by layers), block tables, ragged batches.
+ * KVCache (engine/model.py:149-176) keeps one dense array per sequence instead.
+ *
+ * A pool holds n_pages pages of `page` positions (a power of two, 16..1024) of
+ * every kv head, K and V each [n_pages][Hkv][page][D] row-major, D 128 or 256:
+ *   QVEX_KV_BF16: bf16 values;
+ *   QVEX_KV_INT8: codes c in -127..127, value = scale * c;
+ *   QVEX_KV_FP8:  e4m3 codes (OCP, largest 448), value = scale * c;
+ * the 8-bit formats with one fp32 scale per (page, head, slot): the row's
+ * largest magnitude / 127 (or 448), code = round_to_nearest_even(x * (127 / largest)).
+ * Both quotients and the product are fp32, correctly rounded. A row whose
+ * largest magnitude is below 1e-30 is stored as zeros with scale 0; one that
+ * holds a NaN or an infinity as zeros with scale NaN: it reads back as NaN.
+ *
+ * The rows of a call: B sequences; sequence b has rows cu[b] .. cu[b+1]-1 of the
+ * call's tensors (cu NULL: L rows each, T = B*L), at positions pos[b], pos[b]+1,
+ * ... of the sequence; position p lives in slot p % page of page
+ * table[b*table_stride + p/page]. table, pos and cu are in device memory and are
+ * checked there: row offsets are clamped to 0..T, positions outside
+ * 0 .. table_width*page-1 and pages outside 0 .. n_pages-1 (an unused entry is
+ * -1) hold nothing - they are not written, read as zeros, and attention does
+ * not see them. L is the most rows that a sequence has: a larger count is still
+ * served, by fewer blocks than it deserves. Rows outside every sequence (behind
+ * the last one, for a padded batch) are neither read nor written. Two rows of a
+ * call that name the same position of the same page race.
+ * ------------------------------------------------------------------------ */
+enum qvex_kv_format { QVEX_KV_BF16 = 0, QVEX_KV_INT8 = 1, QVEX_KV_FP8 = 2 };
+
+typedef struct qvex_kv_pages {
+  void* k;            /* [n_pages][Hkv][page][D] bf16 or 8-bit codes, 16-byte aligned */
+  void* v;
+  float* k_scales;    /* [n_pages][Hkv][page], 16-byte aligned; NULL for bf16 */
+  float* v_scales;
+  int n_pages, page, Hkv, D, format;
+} qvex_kv_pages;
+
+typedef struct qvex_kv_rows {
+  const int32_t* table;   /* [B][table_width], rows table_stride entries apart */
+  const int32_t* pos;     /* [B] positions held before the call's rows */
+  const int32_t* cu;      /* [B + 1] row offsets, or NULL */
+  long table_stride;
+  int table_width;
+  int B, L, T;
+} qvex_kv_rows;
+
+/* K and V rows into the pages (KVCache.update, engine/model.py:156-170). k: row t,
+ * head h at k + t*k_token + h*k_head (elements), D consecutive values; v alike. */
+int qvex_paged_append(const qvex_kv_pages* pages, const qvex_kv_rows* rows, const uint16_t* k,
+                      long k_token, long k_head, const uint16_t* v, long v_token, long v_head,
+                      void* stream);
+
+/* qvex_attn_qk_rope over pages: projection rows [Hq x (q | gate) | Hkv x k | Hkv x v],
+ * p_stride elements apart; q and k normalised with q_norm / k_norm, their first
+ * rot_dim dims rotated (NeoX form) by position * freqs[i], i < rot_dim / 2 (fp64:
+ * theta^(-2i / rot_dim); the angle is reduced in fp64, so far positions keep
+ * their digits), q to q_out [T, Hq, D], k and v to the pages. fp32 from the
+ * projection to the one rounding of q_out and of the stored values. */
+int qvex_paged_qk_rope(const qvex_kv_pages* pages, const qvex_kv_rows* rows, const uint16_t* proj,
+                       long p_stride, const uint16_t* q_norm, const uint16_t* k_norm, int Hq,
+                       int rot_dim, const double* freqs, float eps, uint16_t* q_out, void* stream);
+
+/* The rows' positions read back, K and V each [T, Hkv, D] in bf16 or (out_f32) fp32. */
+int qvex_paged_read(const qvex_kv_pages* pages, const qvex_kv_rows* rows, void* k_out, void* v_out,
+                    int out_f32, void* stream);
+
+/* Causal GQA attention of the rows over their sequences' pages: row i of sequence
+ * b sees positions 0 .. pos[b] + i, scores scaled by `scale`, out [T, Hq, D] bf16 (a row
+ * that sees nothing gets zeros; an infinity or a NaN among the values leaves that dim of
+ * the rows that see it not finite, and no other row's). q: row t, head h at q + t*q_token + h*q_head; gate
+ * (or NULL): alike, out times sigmoid(gate). max_keys bounds pos[b] + rows of every
+ * sequence (a larger one is still right, only slower). keys_per_split: keys per
+ * block of a row's split (a multiple of 128), or 0 to choose by the call's size;
+ * at one positive value a row's bits do not depend on the other rows of the call,
+ * as long as the calls have up to 8 rows per sequence.
+ * workspace: qvex_paged_attention_workspace_bytes() of the same arguments,
+ * 16-byte aligned (NULL where that is 0); it need not be cleared. */
+uint64_t qvex_paged_attention_workspace_bytes(int B, int L, int T, int Hq, int Hkv, int D,
+                                              int max_keys, int keys_per_split);
+int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_rows* rows, const uint16_t* q,
+                         long q_token, long q_head, int Hq, int max_keys, int keys_per_split,
+                         const uint16_t* gate, long gate_token, long gate_head, float scale,
+                         uint16_t* out, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Device-side cycle bookkeeping (host side of decode(),
  * engine/speculative.py:82-102), so a whole MTP cycle can be captured once in a
  * HIP graph and replayed with one host synchronisation.

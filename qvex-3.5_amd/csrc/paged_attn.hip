@@ -1,0 +1,521 @@
+// Attention over a paged KV cache (mx.fast.scaled_dot_product_attention with the
+// sigmoid gate, engine/model.py:221-232), pages in bf16 or 8 bits.
+//
+//   o = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale q.k_p - m),  over positions p <= pos + i
+//
+// in one pass with a running reference m and sum, split over the keys and merged.
+// A tile is 16 rows of one kv head: rows (position i, query head of the group),
+// in that order, so that any group size fills it. Both products are transposed:
+//   S^T[keys x rows] = K Q^T: row i of key tile h is key 8 (i / 4) + 4 h + i % 4 of a
+//     32-key block, so that lane (lg, li) ends with keys 8 lg .. 8 lg + 7 of q row li, the B
+//     operand of
+//   O^T[dims x rows] += V^T P^T: lane (lg, li) of tile n holds keys 8 lg .. + 7 of dim
+//     (D / 16) li + n. Those come from row-major pages without a transpose in memory: a
+//     lane loads D / 16 consecutive dims of eight keys (16 lanes a whole row) and
+//     gathers a dim's eight keys from its own registers.
+// So K, V and P never leave their lanes, and a lane owns one q row. Codes are exact in
+// bf16: K's scale multiplies the score, V's the weight. P goes into the second product
+// as two bf16 terms (16 bits of it), so the output's own rounding is the one that shows.
+#include "paged.h"
+
+namespace {
+
+typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pa_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
+typedef float pa_f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int PA_ROWS = 16;            // rows of a tile
+constexpr int PA_STEP = 128;           // keys of a block's step: 32 per wave
+constexpr float PA_NONE = -3.0e38f;    // m before any visible key
+constexpr float PA_SLACK = 8.0f;       // m moves when a score (base 2) passes it by more: P up to 256
+
+struct PaArgs {
+  KvPages c;
+  KvRows r;
+  const uint16_t* q;
+  long q_token, q_head;
+  const uint16_t* gate;
+  long g_token, g_head;
+  uint16_t* out;
+  float* ws;                           // O [T * Hq][nsplit][D], then (m, l) [T * Hq][nsplit]
+  int Hq, kps, nsplit, vec;
+  float c2;                            // scale * log2(e): scores in base 2
+};
+
+__device__ __forceinline__ pa_bf16x8 as_pa8(const u32x4 v) { return __builtin_bit_cast(pa_bf16x8, v); }
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((pa_f32x2{lo, hi}), pa_bf16x2));
+}
+__device__ __forceinline__ float2* pa_ml(const PaArgs& a, int D) {
+  return reinterpret_cast<float2*>(a.ws + (size_t)a.r.T * a.Hq * a.nsplit * D);
+}
+
+// A uniform word of the block table: a scalar load.
+__device__ __forceinline__ int pa_page(const int32_t* t, int i) {
+  return ((const __attribute__((address_space(4))) int32_t*)t)[i];
+}
+
+__device__ __forceinline__ u32x4 pa_load8(const uint16_t* p, int vec) {
+  if (vec) return load16(p);
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  return w;
+}
+
+// Codes e .. e + 7 of eight bytes as bf16.
+template <int FMT>
+__device__ __forceinline__ u32x4 codes8(uint32_t lo, uint32_t hi) {
+  u32x4 o;
+  if constexpr (FMT == QVEX_KV_FP8) {
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  } else {
+    o[0] = pa_pack((float)(int8_t)lo, (float)(int8_t)(lo >> 8));
+    o[1] = pa_pack((float)(int8_t)(lo >> 16), (float)(int8_t)(lo >> 24));
+    o[2] = pa_pack((float)(int8_t)hi, (float)(int8_t)(hi >> 8));
+    o[3] = pa_pack((float)(int8_t)(hi >> 16), (float)(int8_t)(hi >> 24));
+  }
+  return o;
+}
+
+// The A operands of tiles 2 t and 2 t + 1: values 2 t and 2 t + 1 of each of eight keys' runs v.
+template <int FMT, int VW>
+__device__ __forceinline__ void gather2(const uint32_t (&v)[8][VW], int t, u32x4& a0, u32x4& a1) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (FMT == QVEX_KV_BF16) {
+      a0[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x05040100u);
+      a1[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x07060302u);
+    } else {
+      const uint32_t x = v[2 * i][t >> 1], y = v[2 * i + 1][t >> 1];
+      if constexpr (FMT == QVEX_KV_FP8) {
+        const uint32_t w = __builtin_amdgcn_perm(y, x, t & 1 ? 0x07030602u : 0x05010400u);
+        a0[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+        a1[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+      } else {
+        const int s = t & 1 ? 16 : 0;
+        a0[i] = pa_pack((float)(int8_t)(x >> s), (float)(int8_t)(y >> s));
+        a1[i] = pa_pack((float)(int8_t)(x >> (s + 8)), (float)(int8_t)(y >> (s + 8)));
+      }
+    }
+  }
+}
+
+// Whether a word of V holds an infinity or a NaN.
+template <int FMT>
+__device__ __forceinline__ bool wild(uint32_t w) {
+  if constexpr (FMT == QVEX_KV_BF16) return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  if constexpr (FMT == QVEX_KV_FP8) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (w >> (8 * i) & 0x7fu) == 0x7fu;
+    return any;
+  }
+  return false;
+}
+
+__device__ __forceinline__ void pa_gate_store(const PaArgs& a, int t, int h, int d, int D, const float (&o)[4]) {
+  uint16_t* op = a.out + ((size_t)t * a.Hq + h) * D + d;
+  float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+  if (a.gate) {
+    const uint16_t* gp = a.gate + t * a.g_token + h * a.g_head + d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = 1.0f / (1.0f + expf(-bf16_to_f32(gp[i])));
+  }
+  *reinterpret_cast<u32x2*>(op) = u32x2{pack_bf16x2(o[0] * g[0], o[1] * g[1]), pack_bf16x2(o[2] * g[2], o[3] * g[3])};
+}
+
+// One block per (kv head, 16-row tile, sequence, split): its 4 waves take 32 keys each of every
+// 128, alone until their (m, l, O) are merged in LDS.
+template <int FMT, int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
+#pragma clang fp contract(off)
+  constexpr int EB = kv_bytes(FMT), KS = D / 32, KU = D * EB / 64, E = D / 16, VW = E * EB / 4, ROW = D * EB;
+  __shared__ __align__(16) float obuf[4][PA_ROWS][D + 4];
+  __shared__ float2 mlbuf[4][PA_ROWS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int li = lane & 15, lg = lane >> 4;
+  const int b = blockIdx.y, split = blockIdx.z, kh = blockIdx.x % a.c.Hkv, GQ = a.Hq / a.c.Hkv;
+  const KvSeq s(a.r, b);
+  const int cap = a.r.width << a.c.shift, rows = s.n * GQ, mask = (1 << a.c.shift) - 1;
+  const int32_t* table = a.r.table + b * a.r.stride;
+
+  for (int tile = blockIdx.x / a.c.Hkv; tile * PA_ROWS < rows; tile += gridDim.x / a.c.Hkv) {
+    const int row = tile * PA_ROWS + li, last = min(rows, (tile + 1) * PA_ROWS) - 1;
+    const bool used = row < rows;
+    const int i = used ? row / GQ : 0, g = used ? row - i * GQ : 0;
+    const int i_lo = tile * PA_ROWS / GQ, i_hi = last / GQ;       // positions of the tile
+    const int rlim = used ? min(s.pos + i, cap - 1) : -1;
+    const int keys = min(s.pos + i_hi + 1, cap);                  // that any row sees
+    const int k_lo = split * a.kps, k_hi = split == a.nsplit - 1 ? keys : min(k_lo + a.kps, keys);
+    if (k_lo >= k_hi) continue;                                   // uniform; the merge does not read it
+
+    u32x4 qa[KS];
+    const uint16_t* qp = a.q + (s.first + i) * a.q_token + (kh * GQ + g) * a.q_head;
+#pragma unroll
+    for (int st = 0; st < KS; ++st) {
+      const int d = EB == 2 ? 32 * st + 8 * lg : 64 * (st >> 1) + 16 * lg + 8 * (st & 1);
+      qa[st] = used ? pa_load8(qp + d, a.vec) : u32x4{0, 0, 0, 0};
+    }
+
+    u32x4 kr[2][KU];
+    uint32_t vr[8][VW];
+    float ksc[8], vsc[8];
+    bool ok0 = true, ok1 = true;                                  // of the block's two 16-key halves
+    long at0 = 0, at1 = 0;
+    auto locate = [&](int kb) __attribute__((always_inline)) {
+      const int p0 = pa_page(table, min(kb >> a.c.shift, a.r.width - 1));
+      const int p1 = pa_page(table, min((kb + 16) >> a.c.shift, a.r.width - 1));
+      ok0 = p0 >= 0 && p0 < a.c.n_pages;
+      ok1 = p1 >= 0 && p1 < a.c.n_pages;
+      at0 = (((long)(ok0 ? p0 : 0) * a.c.Hkv + kh) << a.c.shift) + (kb & mask);
+      at1 = (((long)(ok1 ? p1 : 0) * a.c.Hkv + kh) << a.c.shift) + ((kb + 16) & mask);
+    };
+    auto load_k = [&]() __attribute__((always_inline)) {
+      const long at = (li >> 3 ? at1 : at0) + 8 * ((li >> 2) & 1) + (li & 3);
+      const uint8_t* p = a.c.k + at * ROW + 16 * lg;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < KU; ++u) kr[h][u] = load16(p + 4 * h * ROW + 64 * u);
+      if constexpr (EB == 1) {
+        const float* sp = a.c.ks + (lg >> 1 ? at1 : at0) + 8 * (lg & 1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ksc[e] = sp[e];
+      }
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
+      const long at = (lg >> 1 ? at1 : at0) + 8 * (lg & 1);
+      const uint8_t* p = a.c.v + at * ROW + li * (4 * VW);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (VW == 2) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(p + e * ROW);
+          vr[e][0] = w[0];
+          vr[e][1] = w[1];
+        } else {
+#pragma unroll
+          for (int u = 0; u < VW / 4; ++u) {
+            const u32x4 w = load16(p + e * ROW + 16 * u);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) vr[e][4 * u + x] = w[x];
+          }
+        }
+      }
+      if constexpr (EB == 1) {
+        const float* sp = a.c.vs + at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vsc[e] = sp[e];
+      }
+    };
+
+    const pa_f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = PA_NONE, l = 0.0f;
+    pa_f32x4 o[E];
+#pragma unroll
+    for (int n = 0; n < E; ++n) o[n] = zero;
+
+    for (int kb = k_lo + 32 * wave; kb < k_hi; kb += PA_STEP) {
+      locate(kb);
+      load_k();
+      load_v();
+      pa_f32x4 sc[2] = {zero, zero};
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4 ka;
+          if constexpr (EB == 2) ka = kr[h][st];
+          else ka = codes8<FMT>(kr[h][st >> 1][2 * (st & 1)], kr[h][st >> 1][2 * (st & 1) + 1]);
+          sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(ka), as_pa8(qa[st]), sc[h], 0, 0, 0);
+        }
+      float t[8], top = -INFINITY;
+      uint32_t vis = 0xff;                                        // of the lane's keys 8 lg ..
+      const bool edge = kb + 32 > min(s.pos + i_lo + 1, k_hi) || !ok0 || !ok1;   // uniform
+      if (edge) {
+        vis = 0;
+        if (lg >> 1 ? ok1 : ok0)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) vis |= (kb + 8 * lg + e <= min(rlim, k_hi - 1) ? 1u : 0u) << e;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        t[e] = sc[e >> 2][e & 3] * a.c2;
+        if constexpr (EB == 1) t[e] *= ksc[e];
+        if (edge && !(vis >> e & 1)) t[e] = -INFINITY;
+        top = fmaxf(top, t[e]);
+      }
+      if (__any(top - m > PA_SLACK)) {
+        float x = fmaxf(top, __shfl_xor(top, 16, 64));
+        x = fmaxf(x, __shfl_xor(x, 32, 64));                      // of the row, in its four lanes
+        const float mn = x - m > PA_SLACK ? x : m;
+        const float f = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int n = 0; n < E; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][j] *= f;
+      }
+      u32x4 p, p_lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        t[e] = __builtin_amdgcn_exp2f(t[e] - m);
+        l += t[e];
+        if constexpr (EB == 1) t[e] = edge && !(vis >> e & 1) ? 0.0f : t[e] * vsc[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = pa_pack(t[2 * e], t[2 * e + 1]);
+        p_lo[e] = pa_pack(t[2 * e] - bf16_lo(p[e]), t[2 * e + 1] - bf16_hi(p[e]));
+      }
+      bool apart = false;
+      if (edge && FMT != QVEX_KV_INT8) {
+        // what no row of the tile sees is not data, and 0 times a NaN or an infinity
+        // is none: keys past the last row's (and pages that are not there) become 0
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = kb + 8 * lg + e;
+          const bool live = key < k_hi && (lg >> 1 ? ok1 : ok0);
+#pragma unroll
+          for (int u = 0; u < VW; ++u) {
+            if (!live) vr[e][u] = 0;
+            any |= key > s.pos + i_lo && wild<FMT>(vr[e][u]);
+          }
+        }
+        apart = __any(any);
+      }
+      if (apart) {
+        // some rows see a NaN or an infinity that others of the tile do not: the keys that
+        // not every row sees are added one by one, and left out of the product
+#pragma unroll 1
+        for (int kg = 0; kg < 4; ++kg) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = kb + 8 * kg + e;
+            if (key <= s.pos + i_lo || key >= k_hi || !(kg >> 1 ? ok1 : ok0)) continue;   // uniform
+            const float w = __shfl(t[e], 16 * kg + li, 64);
+            const uint8_t* p1 = a.c.v + ((kg >> 1 ? at1 : at0) + 8 * (kg & 1) + e) * ROW;
+            if (key <= rlim)
+#pragma unroll
+              for (int n = 0; n < E; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int d = E * (4 * lg + j) + n;
+                  float x;
+                  if constexpr (EB == 2) x = bf16_to_f32(reinterpret_cast<const uint16_t*>(p1)[d]);
+                  else x = __builtin_amdgcn_cvt_f32_fp8((int)p1[d], 0);
+                  o[n][j] = fmaf(w, x, o[n][j]);
+                }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int u = 0; u < VW; ++u)
+            if (kb + 8 * lg + e > s.pos + i_lo) vr[e][u] = 0;
+      }
+#pragma unroll
+      for (int n = 0; n < E; n += 2) {
+        u32x4 a0, a1;
+        gather2<FMT, VW>(vr, n / 2, a0, a1);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(a0), as_pa8(p), o[n], 0, 0, 0);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(a0), as_pa8(p_lo), o[n], 0, 0, 0);
+        o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(a1), as_pa8(p), o[n + 1], 0, 0, 0);
+        o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(a1), as_pa8(p_lo), o[n + 1], 0, 0, 0);
+      }
+    }
+
+    // the waves' sums, merged in the order of the waves
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (used) {
+      if (lg == 0) mlbuf[wave][li] = make_float2(m, l);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int n = 0; n < E; n += 4)                            // dims E (4 lg + j) + n of q row li
+          *reinterpret_cast<float4*>(&obuf[wave][li][E * (4 * lg + j) + n]) =
+              make_float4(o[n][j], o[n + 1][j], o[n + 2][j], o[n + 3][j]);
+    }
+    __syncthreads();
+    const int here = last + 1 - tile * PA_ROWS;
+    for (int x = threadIdx.x; x < here * (D / 4); x += 256) {
+      const int rr = x / (D / 4), d = 4 * (x % (D / 4)), rw = tile * PA_ROWS + rr;
+      const int tok = s.first + rw / GQ, head = kh * GQ + rw % GQ;
+      float mm = PA_NONE;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mlbuf[w][rr].x);
+      float ll = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 ml = mlbuf[w][rr];
+        const float f = __builtin_amdgcn_exp2f(ml.x - mm);
+        const float4 ov = *reinterpret_cast<const float4*>(&obuf[w][rr][d]);
+        ll = fmaf(ml.y, f, ll);
+        acc[0] = fmaf(ov.x, f, acc[0]);
+        acc[1] = fmaf(ov.y, f, acc[1]);
+        acc[2] = fmaf(ov.z, f, acc[2]);
+        acc[3] = fmaf(ov.w, f, acc[3]);
+      }
+      if (a.nsplit == 1) {
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= inv;
+        pa_gate_store(a, tok, head, d, D, acc);
+      } else {
+        const size_t rec = ((size_t)tok * a.Hq + head) * a.nsplit + split;
+        *reinterpret_cast<float4*>(a.ws + rec * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (d == 0) pa_ml(a, D)[rec] = make_float2(mm, ll);
+      }
+    }
+    __syncthreads();
+  }
+
+  // rows of sequences without a visible key (a negative position): nobody else writes them
+  if (a.nsplit == 1 && s.pos < 0) {
+    for (int w = blockIdx.x / a.c.Hkv; w < s.n && s.pos + w < 0; w += gridDim.x / a.c.Hkv)
+      for (int x = threadIdx.x; x < GQ * D; x += 256) a.out[((size_t)(s.first + w) * a.Hq + kh * GQ) * D + x] = 0;
+  }
+}
+
+// A row's records merged in key order, eight requested at a time; D / 4 lanes a row.
+template <int D>
+__global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
+#pragma clang fp contract(off)
+  constexpr int LANES = D / 4, PER = 256 / LANES, BATCH = 8;
+  const int b = blockIdx.y, d = 4 * (threadIdx.x % LANES);
+  const KvSeq s(a.r, b);
+  const int cap = a.r.width << a.c.shift;
+  const long rows = (long)s.n * a.Hq;
+  for (long w = (long)blockIdx.x * PER + threadIdx.x / LANES; w < rows; w += (long)gridDim.x * PER) {
+    const int i = (int)(w / a.Hq), h = (int)(w - (long)i * a.Hq), tok = s.first + i;
+    const int keys = min(s.pos + i + 1, cap);
+    const int act = keys <= 0 ? 0 : min((keys - 1) / a.kps + 1, a.nsplit);
+    const size_t rec = ((size_t)tok * a.Hq + h) * a.nsplit;
+    const float2* mls = pa_ml(a, D) + rec;
+    const float* os = a.ws + rec * D + d;
+    float m = PA_NONE, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < act; s0 += BATCH) {
+      float2 ml[BATCH];
+      float4 ov[BATCH];
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        const int at = min(s0 + x, act - 1);
+        ml[x] = mls[at];
+        ov[x] = *reinterpret_cast<const float4*>(os + (size_t)at * D);
+      }
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        if (s0 + x >= act) break;
+        const float mn = fmaxf(m, ml[x].x);
+        const float fa = __builtin_amdgcn_exp2f(m - mn), fb = __builtin_amdgcn_exp2f(ml[x].x - mn);
+        m = mn;
+        l = fmaf(ml[x].y, fb, l * fa);
+        o[0] = fmaf(ov[x].x, fb, o[0] * fa);
+        o[1] = fmaf(ov[x].y, fb, o[1] * fa);
+        o[2] = fmaf(ov[x].z, fb, o[2] * fa);
+        o[3] = fmaf(ov[x].w, fb, o[3] * fa);
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= inv;
+    pa_gate_store(a, tok, h, d, D, o);
+  }
+}
+
+struct PaPlan {
+  int tiles, kps, nsplit;              // row tiles of the longest sequence; keys per split; splits
+  uint64_t bytes;
+};
+
+bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps, PaPlan* p) {
+  if (B < 1 || L < 1 || T < 0 || Hkv < 1 || Hq < Hkv || Hq % Hkv || (D != 128 && D != 256) || max_keys < 1 ||
+      max_keys > KV_LIMIT || kps < 0 || kps % PA_STEP)
+    return false;
+  const long GQ = Hq / Hkv, tiles = (std::min(L, std::max(T, 1)) * GQ + PA_ROWS - 1) / PA_ROWS;
+  const long steps = (max_keys + PA_STEP - 1) / PA_STEP;
+  if (kps == 0) {
+    const long blocks = std::min(B * tiles, T * GQ / PA_ROWS + B) * Hkv;
+    const long n = std::min(std::max(1024 / std::max(blocks, 1L), 1L), steps);
+    kps = (int)((steps + n - 1) / n) * PA_STEP;
+  }
+  p->tiles = (int)std::min<long>(tiles, 1 << 20);
+  p->kps = kps;
+  p->nsplit = (max_keys - 1) / kps + 1;
+  p->bytes = p->nsplit == 1 ? 0 : (uint64_t)T * Hq * p->nsplit * (D + 2) * sizeof(float);
+  return true;
+}
+
+template <int FMT, int D>
+void launch_attn(dim3 grid, hipStream_t st, const PaArgs& a) {
+  hipLaunchKernelGGL((paged_attn_kernel<FMT, D>), grid, dim3(256), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" uint64_t qvex_paged_attention_workspace_bytes(int B, int L, int T, int Hq, int Hkv, int D, int max_keys,
+                                                         int keys_per_split) {
+  PaPlan p;
+  return pa_plan(B, L, T, Hq, Hkv, D, max_keys, keys_per_split, &p) ? p.bytes : 0;
+}
+
+extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_rows* rows, const uint16_t* q,
+                                    long q_token, long q_head, int Hq, int max_keys, int keys_per_split,
+                                    const uint16_t* gate, long gate_token, long gate_head, float scale, uint16_t* out,
+                                    void* workspace, uint64_t workspace_bytes, void* stream) {
+  const char* fn = "qvex_paged_attention";
+  PaArgs a;
+  if (const int rc = kv_check(fn, pages, rows, &a.c, &a.r)) return rc;
+  const int B = rows->B, D = pages->D;
+  PaPlan p;
+  QVEX_CHECK_ARG(pa_plan(B, a.r.L, a.r.T, Hq, a.c.Hkv, D, max_keys, keys_per_split, &p) && Hq <= 16384,
+                 "%s: Hq=%d Hkv=%d max_keys=%d keys_per_split=%d (a multiple of 128, or 0)", fn, Hq, a.c.Hkv, max_keys,
+                 keys_per_split);
+  QVEX_CHECK_ARG(p.nsplit <= 65535, "%s: grid too large", fn);
+  if (a.r.T == 0) return QVEX_OK;
+  QVEX_CHECK_ARG(q && out && qvex_aligned(q, 2) && qvex_aligned(out, 16) && qvex_aligned(gate, 2),
+                 "%s: null or misaligned q, gate or out (out 16-byte aligned)", fn);
+  QVEX_CHECK_ARG(workspace_bytes >= p.bytes && (p.bytes == 0 || (workspace && qvex_aligned(workspace, 16))),
+                 "%s: workspace %llu < %llu bytes, or not 16-byte aligned", fn, (unsigned long long)workspace_bytes,
+                 (unsigned long long)p.bytes);
+  a.q = q;
+  a.q_token = q_token;
+  a.q_head = q_head;
+  a.gate = gate;
+  a.g_token = gate_token;
+  a.g_head = gate_head;
+  a.out = out;
+  a.ws = (float*)workspace;
+  a.Hq = Hq;
+  a.kps = p.kps;
+  a.nsplit = p.nsplit;
+  a.vec = (q_token % 8 | q_head % 8) == 0 && qvex_aligned(q, 16);
+  a.c2 = scale * 1.44269504088896340736f;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid(a.c.Hkv * p.tiles, B, p.nsplit);
+  const int f = pages->format;
+  const auto go = D == 256 ? (f == QVEX_KV_BF16   ? &launch_attn<QVEX_KV_BF16, 256>
+                              : f == QVEX_KV_INT8 ? &launch_attn<QVEX_KV_INT8, 256>
+                                                  : &launch_attn<QVEX_KV_FP8, 256>)
+                           : (f == QVEX_KV_BF16   ? &launch_attn<QVEX_KV_BF16, 128>
+                              : f == QVEX_KV_INT8 ? &launch_attn<QVEX_KV_INT8, 128>
+                                                  : &launch_attn<QVEX_KV_FP8, 128>);
+  go(grid, st, a);
+  QVEX_CHECK_LAUNCH(fn);
+  if (p.nsplit > 1) {
+    const int per = 256 / (D / 4);
+    const long most = (8192 + B - 1) / B, want = ((long)a.r.L * Hq + per - 1) / per;
+    const dim3 mgrid((unsigned)std::min(want, most), B);
+    if (D == 256) hipLaunchKernelGGL(paged_attn_merge_kernel<256>, mgrid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(paged_attn_merge_kernel<128>, mgrid, dim3(256), 0, st, a);
+    QVEX_CHECK_LAUNCH("qvex_paged_attention/merge");
+  }
+  return QVEX_OK;
+}

@@ -17,6 +17,19 @@ U64 = ctypes.c_uint64
 F = ctypes.c_float
 LNG = ctypes.c_long
 
+
+class KvPages(ctypes.Structure):
+    """qvex_kv_pages"""
+    _fields_ = [("k", P), ("v", P), ("k_scales", P), ("v_scales", P), ("n_pages", I), ("page", I), ("Hkv", I), ("D", I),
+                ("format", I)]
+
+
+class KvRows(ctypes.Structure):
+    """qvex_kv_rows"""
+    _fields_ = [("table", P), ("pos", P), ("cu", P), ("table_stride", LNG), ("table_width", I), ("B", I), ("L", I),
+                ("T", I)]
+
+
 # name -> argtypes (all return int status)
 SIGNATURES: dict[str, list] = {
     "qvex_qmv_w4g64": [P, P, P, P, P, I, I, I, P],
@@ -76,6 +89,10 @@ SIGNATURES: dict[str, list] = {
     "qvex_attention": [P, P, P, P, I, I, I, I, I, I, I, I, P, LNG, P, P, U64, P],
     "qvex_attention_decode": [P, LNG, P, P, P, I, I, I, I, I, F, P, I, P, P, I, I, I, P, P, U64, P],
     "qvex_rope_table": [I, F, I, P, P],
+    "qvex_paged_append": [P, P, P, LNG, LNG, P, LNG, LNG, P],
+    "qvex_paged_qk_rope": [P, P, P, LNG, P, P, I, I, P, F, P, P],
+    "qvex_paged_read": [P, P, P, P, I, P],
+    "qvex_paged_attention": [P, P, P, LNG, LNG, I, I, I, P, LNG, LNG, F, P, P, U64, P],
 }
 
 # qvex_abi_version() of the library these bindings match (8: the RoPE table of
@@ -118,6 +135,8 @@ def lib() -> ctypes.CDLL:
         L.qvex_sampler_scores_workspace_bytes.argtypes = [I, I, I]
         L.qvex_qmv_w4g64_argmax_workspace_bytes.restype = U64
         L.qvex_qmv_w4g64_argmax_workspace_bytes.argtypes = [I, I]
+        L.qvex_paged_attention_workspace_bytes.restype = U64
+        L.qvex_paged_attention_workspace_bytes.argtypes = [I, I, I, I, I, I, I, I]
         L.qvex_spec_accept_tiles_applies.restype = I          # 1 / 0, not a status
         L.qvex_spec_accept_tiles_applies.argtypes = [I, I, I, F, I, F]
         for name, args in SIGNATURES.items():
@@ -141,4 +160,4 @@ def exported_symbols() -> list[str]:
             "qvex_attn_workspace_bytes", "qvex_w4g64_packed_bytes",
             "qvex_gdn_chunked_workspace_bytes", "qvex_spec_accept_filtered_workspace_bytes",
             "qvex_qmv_w4g64_argmax_workspace_bytes", "qvex_sampler_scores_workspace_bytes",
-            "qvex_spec_accept_tiles_applies", *SIGNATURES]
+            "qvex_spec_accept_tiles_applies", "qvex_paged_attention_workspace_bytes", *SIGNATURES]

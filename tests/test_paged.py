@@ -1,0 +1,178 @@
+"""Paged KV cache on the CPU: what the entry points and their front end refuse, before any GPU work."""
+
+import ctypes
+
+import pytest
+import torch
+
+from qvex import _C, paged
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture()
+def buf():
+    b = ctypes.create_string_buffer(1 << 12)
+    yield (ctypes.addressof(b) + 15) // 16 * 16
+    del b
+
+
+def pages_of(p, **kw):
+    f = {"k": p, "v": p, "k_scales": p, "v_scales": p, "n_pages": 4, "page": 64, "Hkv": 2, "D": 128, "format": 1, **kw}
+    return _C.KvPages(*f.values())
+
+
+def rows_of(p, **kw):
+    f = {"table": p, "pos": p, "cu": p, "table_stride": 4, "table_width": 4, "B": 2, "L": 3, "T": 5, **kw}
+    return _C.KvRows(*f.values())
+
+
+def calls(p, pages, rows):
+    """Every entry point on these structs."""
+    a, b = ctypes.byref(pages), ctypes.byref(rows)
+    return {"qvex_paged_append": (a, b, p, 256, 128, p, 256, 128, None),
+            "qvex_paged_qk_rope": (a, b, p, 4 * 2 * 128 + 4 * 128, p, p, 4, 32, p, 1e-6, p, None),
+            "qvex_paged_read": (a, b, p, p, 0, None),
+            "qvex_paged_attention": (a, b, p, 512, 128, 4, 100, 0, None, 0, 0, 0.1, p, p, 1 << 30, None)}
+
+
+@pytest.mark.parametrize("kw,match", [
+    ({"format": 3}, "format"), ({"format": -1}, "format"), ({"D": 64}, "D=64"), ({"page": 48}, "page=48"),
+    ({"page": 8}, "page=8"), ({"page": 2048}, "page=2048"), ({"n_pages": 0}, "n_pages"), ({"Hkv": 0}, "Hkv=0"),
+    ({"k": None}, "16-byte"), ({"v_scales": None}, "scales"),
+])
+def test_every_entry_point_refuses_bad_pages(buf, kw, match):
+    for name, args in calls(buf, pages_of(buf, **kw), rows_of(buf)).items():
+        with pytest.raises(_C.QvexError, match=f"{name}.*{match}"):
+            _C.call(name, *args)
+
+
+def test_every_entry_point_refuses_misaligned_pages(buf):
+    for name, args in calls(buf, pages_of(buf, k=buf + 8), rows_of(buf)).items():
+        with pytest.raises(_C.QvexError, match="16-byte"):
+            _C.call(name, *args)
+
+
+@pytest.mark.parametrize("kw,match", [
+    ({"B": 0}, "B=0"), ({"B": 70000}, "B=70000"), ({"L": 0}, "L=0"), ({"T": -1}, "T=-1"), ({"T": 1 << 30}, "T="),
+    ({"cu": None}, "T=5"), ({"table": None}, "table"), ({"pos": None}, "positions"), ({"table_width": 0}, "table_width"),
+    ({"table_stride": 3}, "table_stride"), ({"table_width": 1 << 25, "table_stride": 1 << 25}, "table_width"),
+])
+def test_every_entry_point_refuses_bad_rows(buf, kw, match):
+    for name, args in calls(buf, pages_of(buf), rows_of(buf, **kw)).items():
+        with pytest.raises(_C.QvexError, match=f"{name}.*{match}"):
+            _C.call(name, *args)
+
+
+def test_null_structs_are_refused(buf):
+    for name, args in calls(buf, pages_of(buf), rows_of(buf)).items():
+        with pytest.raises(_C.QvexError, match="null"):
+            _C.call(name, None, *args[1:])
+        with pytest.raises(_C.QvexError, match="null"):
+            _C.call(name, args[0], None, *args[2:])
+
+
+def edited(args, **at):
+    out = list(args)
+    for i, v in at.items():
+        out[int(i[1:])] = v
+    return out
+
+
+@pytest.mark.parametrize("name,at,match", [
+    ("qvex_paged_append", {"_2": None}, "null"), ("qvex_paged_append", {"_5": None}, "null"),
+    ("qvex_paged_qk_rope", {"_2": None}, "null"), ("qvex_paged_qk_rope", {"_3": 100}, "p_stride"),
+    ("qvex_paged_qk_rope", {"_6": 3}, "Hq=3"), ("qvex_paged_qk_rope", {"_7": 33}, "rot_dim"),
+    ("qvex_paged_qk_rope", {"_7": 130}, "rot_dim"), ("qvex_paged_qk_rope", {"_8": None}, "null"),
+    ("qvex_paged_read", {"_2": None}, "aligned"), ("qvex_paged_attention", {"_2": None}, "null"),
+    ("qvex_paged_attention", {"_5": 5}, "Hq=5"), ("qvex_paged_attention", {"_6": 0}, "max_keys"),
+    ("qvex_paged_attention", {"_7": 100}, "keys_per_split"), ("qvex_paged_attention", {"_7": -128}, "keys_per_split"),
+    ("qvex_paged_attention", {"_6": 5000, "_7": 128, "_14": 1000}, "workspace"),
+    ("qvex_paged_attention", {"_6": 5000, "_7": 128, "_13": None}, "workspace"), ("qvex_paged_attention", {"_12": None}, "null"),
+])
+def test_bad_arguments_are_refused(buf, name, at, match):
+    args = edited(calls(buf, pages_of(buf), rows_of(buf))[name], **at)
+    with pytest.raises(_C.QvexError, match=match):
+        _C.call(name, *args)
+
+
+def test_workspace_bytes():
+    f = _C.lib().qvex_paged_attention_workspace_bytes
+    assert f(2, 3, 5, 4, 2, 128, 100, 0) == 0                       # one split
+    assert f(1, 1, 1, 16, 4, 256, 4096, 128) == 16 * 32 * 258 * 4
+    assert f(1, 1, 1, 16, 3, 256, 4096, 128) == 0 and f(1, 1, 1, 16, 4, 64, 4096, 128) == 0     # refused shapes
+    # a workspace of a call serves calls of fewer keys
+    for kps in (0, 128, 512):
+        sizes = [f(3, 4, 9, 8, 2, 128, mk, kps) for mk in range(1, 5000, 77)]
+        assert kps == 0 or sizes == sorted(sizes)
+
+
+def test_front_end_refuses_host_tensors():
+    k = torch.zeros((2, 2, 16, 128), dtype=torch.int8)
+    with pytest.raises(_C.QvexError, match="GPU tensor"):
+        paged.KVPages(k, k, torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16)))
+    with pytest.raises(_C.QvexError, match="bf16, int8"):
+        paged.KVPages(k.float(), k.float())
+    with pytest.raises(_C.QvexError, match="unknown KV format"):
+        paged.KVPages.alloc(2, 2, 128, "int4")
+
+
+class _FakePages(paged.KVPages):
+    """A handle over host memory, for the checks that run before a launch."""
+
+    def __init__(self):
+        self.fmt, self.n_pages, self.n_kv, self.page, self.head_dim = "int8", 4, 2, 16, 128
+        self.device = torch.device("cpu")
+        self._ref = None
+
+    def _stream(self):
+        raise AssertionError("a refused call reached the launch")
+
+
+def good():
+    z = torch.zeros
+    return {"x": z((6, 2, 128), dtype=BF16), "table": z((2, 4), dtype=torch.int32), "pos": z(2, dtype=torch.int32),
+            "cu": torch.tensor([0, 2, 6], dtype=torch.int32), "proj": z((6, 4 * 2 * 128 + 4 * 128), dtype=BF16),
+            "w": z(128, dtype=BF16), "freqs": z(16, dtype=torch.float64)}
+
+
+@pytest.mark.parametrize("key,value,match", [
+    ("x", torch.zeros((6, 2, 128)), "bf16"), ("x", torch.zeros((6, 3, 128), dtype=BF16), "kv heads|must be bf16"),
+    ("x", torch.zeros((6, 2, 64), dtype=BF16), "128"), ("x", torch.zeros((6, 2, 256), dtype=BF16)[..., ::2], "consecutive"),
+    ("table", torch.zeros((2, 4)), "table"), ("table", torch.zeros((3, 4), dtype=torch.int32), "table"),
+    ("table", torch.zeros((2, 8), dtype=torch.int32)[:, ::2], "table"), ("pos", torch.zeros(2), "pos"),
+    ("pos", torch.zeros((2, 1), dtype=torch.int32), "pos"), ("cu", torch.zeros(2, dtype=torch.int32), "cu"),
+    ("cu", torch.zeros(3, dtype=torch.int64), "cu"),
+])
+def test_front_end_refuses_bad_tensors(key, value, match):
+    a = {**good(), key: value}
+    pages = _FakePages()
+    with pytest.raises(_C.QvexError, match=match):
+        paged.kv_append(pages, a["x"], a["x"], a["table"], a["pos"], a["cu"])
+    with pytest.raises(_C.QvexError, match=match):
+        paged.attention(pages, a["x"], a["table"], a["pos"], cu=a["cu"])
+    if key != "x":
+        with pytest.raises(_C.QvexError, match=match):
+            paged.kv_read(pages, a["table"], a["pos"], 6, a["cu"])
+        with pytest.raises(_C.QvexError, match=match):
+            paged.attn_qk_rope(pages, a["proj"], a["w"], a["w"], a["table"], a["pos"], a["freqs"], 1e-6, a["cu"])
+
+
+@pytest.mark.parametrize("key,value,match", [
+    ("proj", torch.zeros((6, 1000), dtype=BF16), "rows of 1000"), ("proj", torch.zeros((6, 1536)), "proj"),
+    ("w", torch.zeros(64, dtype=BF16), "norm"), ("freqs", torch.zeros(16), "fp64"),
+])
+def test_front_end_refuses_bad_input_stage(key, value, match):
+    a = {**good(), key: value}
+    with pytest.raises(_C.QvexError, match=match):
+        paged.attn_qk_rope(_FakePages(), a["proj"], a["w"], a["w"], a["table"], a["pos"], a["freqs"], 1e-6, a["cu"])
+
+
+def test_front_end_refuses_rows_without_offsets():
+    a = good()
+    with pytest.raises(_C.QvexError, match="do not divide"):
+        paged.kv_append(_FakePages(), a["x"][:5], a["x"][:5], a["table"], a["pos"])
+    with pytest.raises(_C.QvexError, match="bf16 or fp32"):
+        paged.kv_read(_FakePages(), a["table"], a["pos"], 6, dtype=torch.float16)
+    with pytest.raises(_C.QvexError, match="out must"):
+        paged.attention(_FakePages(), a["x"], a["table"], a["pos"], out=torch.zeros((6, 2, 128)))

@@ -1,0 +1,460 @@
+"""Paged KV cache on the GPU against its definitions on the CPU: append, read-back,
+the attention block's input stage, and attention, at ragged batches, pages that end
+inside a block, unused and wrong table entries, masked NaNs, strides and graphs."""
+
+import math
+
+import pytest
+import torch
+
+import paged_ref as ref
+from qvex import paged
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["bf16", "int8", "fp8"]
+BF16 = torch.bfloat16
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def on(dev, *ts):
+    out = [None if t is None else t.to(dev) for t in ts]
+    return out[0] if len(out) == 1 else out
+
+
+def gpu_pool(pool, dev):
+    return paged.KVPages(*on(dev, pool.k, pool.v), *(() if pool.ks is None else on(dev, pool.ks, pool.vs)))
+
+
+def same_bits(a, b):
+    a, b = a.cpu(), b.cpu()
+    if a.dtype in (torch.float8_e4m3fn,):
+        return torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    return torch.equal(torch.nan_to_num(a.float(), nan=7e9), torch.nan_to_num(b.float(), nan=7e9))
+
+
+def layout(lens, pos, page, seed, spare=3, extra_width=1):
+    """A table of shuffled pages for sequences of pos + lens positions, -1 behind them; its pool's size."""
+    need = [max(0, -(-(p + n) // page)) for p, n in zip(pos, lens)]
+    perm = torch.randperm(sum(need) + spare, generator=gen(seed)).to(torch.int32)
+    table = torch.full((len(lens), max(1, max(need)) + extra_width), -1, dtype=torch.int32)
+    j = 0
+    for b, m in enumerate(need):
+        table[b, :m] = perm[j:j + m]
+        j += m
+    return table, sum(need) + spare
+
+
+def offsets(lens):
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return cu
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+# ---------------------------------------------------------------- append and read
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,n_kv,page,lens,pos", [
+    (256, 4, 64, [1], [0]), (256, 4, 64, [4], [4093]), (128, 2, 16, [5, 0, 33, 1], [0, 7, 30, 15]),
+    (256, 1, 32, [70, 3], [0, 1000]), (128, 8, 1024, [9, 17], [1020, 3]), (256, 3, 16, [1, 1, 1, 1, 1], [0, 15, 16, 31, 32]),
+])
+def test_append_and_read(dev, fmt, D, n_kv, page, lens, pos):
+    """Codes, scales and every untouched slot as defined, bit for bit; read-back is code * scale rounded once."""
+    g = gen(1)
+    T = sum(lens)
+    table, n_pages = layout(lens, pos, page, 2)
+    pool = ref.Pool(n_pages, n_kv, page, D, fmt)
+    # k and v as columns of one projection's rows, with a few rows of other magnitudes
+    kv = torch.randn((T, 2 * n_kv, D), generator=g) * torch.exp2(torch.randint(-20, 20, (T, 2 * n_kv, 1), generator=g).float())
+    kv = kv.to(BF16)
+    k, v = kv[:, :n_kv], kv[:, n_kv:]
+    pages = gpu_pool(pool, dev)
+    cu = offsets(lens)
+    kvd = kv.to(dev)
+    args = (i32(table.tolist(), dev), i32(pos, dev), i32(cu, dev))
+    paged.kv_append(pages, kvd[:, :n_kv], kvd[:, n_kv:], *args)
+    ref.append(pool, k, v, table.tolist(), pos, cu)
+    for got, want in zip(pages.tensors(), pool.tensors()):
+        assert same_bits(got, want)
+    for dtype in (BF16, torch.float32):
+        got = paged.kv_read(pages, args[0], args[1], T, args[2], dtype=dtype)
+        for x, y in zip(got, ref.read(pool, table.tolist(), pos, T, cu)):
+            assert torch.equal(x.cpu(), y.to(dtype))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_append_rows_that_are_not_numbers(dev, fmt):
+    """Zero rows, rows below the smallest scale, NaN and infinite values: in 8 bits the whole row reads back as NaN."""
+    D, n_kv, page = 128, 2, 16
+    x = torch.randn((6, n_kv, D), generator=gen(3)).to(BF16)
+    x[0] = 0.0
+    x[1] = 1e-35
+    x[2, 0, 5] = math.nan
+    x[3, 1, 7] = -math.inf
+    x[4, 0, 0] = torch.finfo(BF16).max
+    pool = ref.Pool(2, n_kv, page, D, fmt)
+    pages = gpu_pool(pool, dev)
+    table, pos = i32([[1, 0]], dev), i32([3], dev)
+    paged.kv_append(pages, x.to(dev), x.flip(0).contiguous().to(dev), table, pos)
+    ref.append(pool, x, x.flip(0), [[1, 0]], [3])
+    for got, want in zip(pages.tensors(), pool.tensors()):
+        assert same_bits(got, want)
+    k, _ = paged.kv_read(pages, table, pos, 6)
+    if fmt != "bf16":
+        assert bool(k[2, 0].isnan().all()) and not bool(k[2, 1].isnan().any()) and bool(k[3, 1].isnan().all())
+    assert bool((k[0] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_append_and_read_where_no_page_is(dev, fmt):
+    """Negative positions, positions past the table, entries outside the pool and padded rows: nothing
+    is written there, zeros are read, and rows outside every sequence stay as they are."""
+    D, n_kv, page = 256, 2, 16
+    table = [[2, 99], [-7, 0], [1, 3]]
+    pos, cu, T = [8, 10, -3], [0, 12, 20, 28], 31
+    x = torch.randn((T, n_kv, D), generator=gen(4)).to(BF16)
+    pool = ref.Pool(4, n_kv, page, D, fmt)
+    pages = gpu_pool(pool, dev)
+    args = (i32(table, dev), i32(pos, dev))
+    paged.kv_append(pages, x.to(dev), (-x).to(dev), *args, i32(cu, dev), max_rows=12)
+    ref.append(pool, x, -x, table, pos, cu)
+    for got, want in zip(pages.tensors(), pool.tensors()):
+        assert same_bits(got, want)
+    k, v = (torch.full((T, n_kv, D), 5.0, dtype=BF16, device=dev) for _ in range(2))
+    paged.kv_read(pages, *args, T, i32(cu, dev), k_out=k, v_out=v)
+    wk, wv = ref.read(pool, table, pos, T, cu, fill=5.0)
+    assert torch.equal(k.cpu(), wk.to(BF16)) and torch.equal(v.cpu(), wv.to(BF16))
+
+
+def test_append_strides_and_row_bound(dev):
+    """Rows and heads of any stride (odd ones too), and a row bound below the longest sequence."""
+    D, n_kv, page, T = 128, 2, 32, 50
+    flat = torch.randn(T * 300 + 7, generator=gen(5)).to(BF16).to(dev)
+    k = flat[3:].as_strided((T, n_kv, D), (277, 133, 1))
+    v = flat[1:].as_strided((T, n_kv, D), (261, 129, 1))
+    pool = ref.Pool(3, n_kv, page, D, "int8")
+    pages = gpu_pool(pool, dev)
+    table = [[2, 0], [1, -1]]
+    paged.kv_append(pages, k, v, i32(table, dev), i32([0, 0], dev), i32([0, 45, 50], dev), max_rows=1)
+    ref.append(pool, k.cpu(), v.cpu(), table, [0, 0], [0, 45, 50])
+    for got, want in zip(pages.tensors(), pool.tensors()):
+        assert same_bits(got, want)
+
+
+# ---------------------------------------------------------------- input stage
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,Hq,n_kv,rot,lens,pos,pad", [
+    (256, 16, 4, 64, [4], [4096], 0), (128, 4, 2, 32, [3, 20, 1], [0, 100, 1000000], 1), (128, 2, 2, 0, [2], [5], 0),
+    (128, 3, 1, 20, [7], [31], 0), (256, 8, 2, 256, [5], [77], 8),
+])
+def test_qk_rope(dev, fmt, D, Hq, n_kv, rot, lens, pos, pad):
+    """q, and what the pages then stand for, against float64: q and bf16 rows one rounding
+    (2^-8), int8 half a scale, fp8 2^-4 or half its smallest step; the fp32 chain
+    (sum of squares, rsqrt, rotation of an angle reduced in fp64) adds 2^-19 of the row's largest."""
+    g = gen(6)
+    T, width = sum(lens), Hq * 2 * D + 2 * n_kv * D
+    proj = torch.randn((T, width + pad), generator=g).to(BF16)[:, :width]
+    qn, kn = (1.0 + 0.2 * torch.randn(D, generator=g)).to(BF16), (1.0 + 0.2 * torch.randn(D, generator=g)).to(BF16)
+    page = 16
+    tab = torch.full((len(lens), max(p + n for p, n in zip(pos, lens)) // page + 1), -1, dtype=torch.int32)
+    j = 0
+    for b, (p, n) in enumerate(zip(pos, lens)):
+        for x in range(p // page, (p + n - 1) // page + 1):
+            tab[b, x] = j
+            j += 1
+    pages = gpu_pool(ref.Pool(j, n_kv, page, D, fmt), dev)
+    freqs = paged.rope_freqs(rot, 1e7, dev) if rot else None
+    cu = offsets(lens)
+    pd = torch.zeros((T, width + pad), dtype=BF16, device=dev)
+    pd[:, :width] = proj.to(dev)
+    args = (tab.to(dev), i32(pos, dev))
+    q = paged.attn_qk_rope(pages, pd[:, :width], qn.to(dev), kn.to(dev), *args, freqs, 1e-6, i32(cu, dev))
+    at = torch.cat([p + torch.arange(n) for p, n in zip(pos, lens)])
+    fr = freqs.cpu() if rot else torch.zeros(0, dtype=torch.float64)
+    wq, wk, wv = ref.qk_rope(proj, qn, kn, Hq, n_kv, D, fr, 1e-6, at)
+
+    def near(got, want, rounding, floor=0.0):
+        far = (got.cpu().double() - want).abs()
+        assert bool((far <= rounding * want.abs() + floor + 2.0 ** -19 * want.abs().amax(dim=-1, keepdim=True)).all())
+
+    near(q, wq, 2.0 ** -8)
+    k, v = paged.kv_read(pages, *args, T, i32(cu, dev), dtype=torch.float32)
+    for got, want in ((k, wk), (v, wv)):
+        top = want.abs().amax(dim=-1, keepdim=True)
+        if fmt == "bf16":
+            near(got, want, 2.0 ** -8)
+        elif fmt == "int8":
+            near(got, want, 0.0, top / 254)
+        else:
+            near(got, want, 2.0 ** -4, top / 448 * 2.0 ** -10)
+
+
+def test_qk_rope_values_are_appended_as_append_does(dev):
+    """v goes to the pages with the bits of kv_append."""
+    D, Hq, n_kv, T, page = 256, 4, 2, 9, 16
+    proj = torch.randn((T, Hq * 2 * D + 2 * n_kv * D), generator=gen(7)).to(BF16).to(dev)
+    w = torch.ones(D, dtype=BF16, device=dev)
+    a, b = (paged.KVPages.alloc(2, n_kv, D, "int8", page, dev) for _ in range(2))
+    table, pos = i32([[1, 0]], dev), i32([11], dev)
+    paged.attn_qk_rope(a, proj, w, w, table, pos, paged.rope_freqs(64, 1e7, dev), 1e-6)
+    v = proj[:, -n_kv * D:].view(T, n_kv, D)
+    paged.kv_append(b, v, v, table, pos)
+    assert torch.equal(a.v, b.v) and torch.equal(a.v_scale, b.v_scale)
+
+
+# ---------------------------------------------------------------- attention
+
+def check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, *, gate=False, scale=None, seed=8, poison=True, kps=0,
+                    max_keys=None, max_rows=None, pad=0, fill_gain=1.0, edit=None):
+    g = gen(seed)
+    T = sum(lens) + pad
+    table, n_pages = layout(lens, pos, page, seed + 1)
+    pool = ref.Pool(n_pages, n_kv, page, D, fmt)
+    if poison:          # what no sequence holds is no data
+        if fmt == "bf16":
+            pool.k[:], pool.v[:] = math.nan, math.inf
+        else:
+            pool.ks[:], pool.vs[:] = math.nan, math.inf
+            if fmt == "fp8":
+                pool.k[:], pool.v[:] = math.nan, math.nan
+    for b, (p, n) in enumerate(zip(pos, lens)):
+        for x in range(max(0, p + n)):
+            at = pool.slot(table[b].tolist(), x)
+            pool.put(at, fill_gain * torch.randn((n_kv, D), generator=g), torch.randn((n_kv, D), generator=g))
+    q = torch.randn((T, Hq, D), generator=g).to(BF16)
+    gt = torch.randn((T, Hq, 2 * D), generator=g).to(BF16) if gate else None
+    cu = offsets(lens)
+    tab = table.tolist()
+    if edit is not None:
+        edit(pool, q, tab)
+    out = torch.full((T, Hq, D), 9.0, dtype=BF16, device=dev)
+    gd = gt.to(dev) if gate else None
+    pages = gpu_pool(pool, dev)
+    paged.attention(pages, q.to(dev), i32(tab, dev), i32(pos, dev), max_keys, i32(cu, dev), max_rows,
+                    gd[..., D:] if gate else None, scale, out, keys_per_split=kps)
+    want, tol = ref.attention(pool, q, tab, pos, cu, gt[..., D:] if gate else None, scale, fill=9.0)
+    got = out.cpu().double()
+    assert torch.equal(got.isfinite(), want.isfinite())
+    fin = want.isfinite()
+    far = (got - want).abs()[fin]
+    assert bool((far <= tol[fin]).all()), f"{float((far - tol[fin]).max())} over at {float(far.max())}"
+    return got, want
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,Hq,n_kv,page,lens,pos", [
+    (256, 16, 4, 64, [1], [0]), (256, 16, 4, 64, [1], [700]), (256, 16, 4, 16, [4], [333]), (256, 8, 2, 32, [8], [127]),
+    (128, 4, 2, 16, [1, 3, 0, 20], [0, 130, 50, 14]), (128, 8, 8, 64, [2, 1], [95, 31]), (128, 6, 2, 128, [5], [250]),
+    (128, 24, 1, 16, [3], [40]), (256, 16, 1, 256, [40], [300]), (128, 4, 2, 32, [130, 1, 65], [0, 200, 63]),
+    (256, 4, 4, 64, [70], [0]),
+])
+def test_attention(dev, fmt, D, Hq, n_kv, page, lens, pos):
+    check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kps,max_keys", [(128, None), (256, 1200), (0, 1), (128, 130), (1152, None)])
+def test_attention_splits(dev, fmt, kps, max_keys):
+    """Any split, and a bound on the keys that is too small."""
+    check_attention(dev, fmt, 128, 4, 2, 64, [2, 1, 9], [1100, 511, 256], kps=kps, max_keys=max_keys, gate=True)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attention_gate_scale_padding(dev, fmt):
+    check_attention(dev, fmt, 256, 8, 4, 32, [3, 12], [77, 0], gate=True, scale=0.02, pad=4)
+    check_attention(dev, fmt, 128, 4, 2, 16, [3, 40], [77, 0], max_rows=1, fill_gain=30.0)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("long", [False, True])
+def test_attention_rows_that_see_nothing(dev, fmt, long):
+    """Negative positions and pages that are not there; a row without any key gets zeros."""
+    n = 70 if long else 6
+
+    def edit(pool, q, tab):
+        tab[0][0] = -1                          # the first page of sequence 0
+        tab[2] = [99] * len(tab[2])
+
+    got, _ = check_attention(dev, fmt, 128, 4, 2, 16, [n, n, n], [5, -4, 20], edit=edit)
+    assert bool((got[n:n + 4] == 0).all()) and bool((got[2 * n:3 * n] == 0).all()) and bool((got[:min(n, 11)] == 0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,Hq,n_kv,n", [(256, 16, 4, 4), (128, 4, 2, 40), (256, 4, 2, 90), (128, 16, 1, 3)])
+def test_attention_nan_and_inf_stay_with_the_rows_that_see_them(dev, fmt, D, Hq, n_kv, n):
+    """A key or value that is not a number, seen by later rows only; a query that is not one."""
+    pos = 61
+
+    def edit(pool, q, tab):
+        k, v = (torch.randn((n_kv, D), generator=gen(10 + i)) for i in range(2))
+        k2, v2 = k.clone(), v.clone()
+        v2[0, 3] = math.nan
+        pool.put(pool.slot(tab[0], pos + n // 2), k, v2)
+        v2 = v.clone()
+        v2[-1, 7] = math.inf
+        pool.put(pool.slot(tab[0], pos + n // 2 + 1), k2, v2)
+        k2[0, 1] = math.nan
+        pool.put(pool.slot(tab[0], pos + n - 1), k2, v)
+        q[1, 0, 5] = math.nan
+
+    _, want = check_attention(dev, fmt, D, Hq, n_kv, 16, [n], [pos], edit=edit)
+    assert bool(want[0].isfinite().all()) and not bool(want[n - 1].isfinite().all())
+
+
+def test_attention_strided_queries_and_workspace(dev):
+    """q and gate as columns of projection rows (odd strides too), a caller's workspace, another stream."""
+    D, Hq, n_kv, page, T, p = 128, 4, 2, 32, 5, 400
+    pages = paged.KVPages(*(torch.randn((14, n_kv, page, D), device=dev).to(BF16) for _ in range(2)))
+    table, pos = i32([list(range(13, -1, -1))], dev), i32([p], dev)
+    proj = torch.randn((T, Hq * 2 * D + 3), device=dev).to(BF16)
+    qg = proj[:, :Hq * 2 * D].unflatten(1, (Hq, 2 * D))
+    q, gate = qg[..., :D], qg[..., D:]
+    want = paged.attention(pages, q.contiguous(), table, pos, gate=gate.contiguous())
+    need = paged.workspace_bytes(pages, 1, T, Hq, 14 * page)
+    ws = torch.full(((need + 3) // 4,), math.nan, device=dev)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = paged.attention(pages, q, table, pos, gate=gate, workspace=ws)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_keep_their_bits_in_calls_of_up_to_8(dev, fmt):
+    """At one keys_per_split a row's result does not depend on the rows it comes with."""
+    D, Hq, n_kv, page, p = 256, 16, 4, 64, 900
+    pages = paged.KVPages.alloc(16, n_kv, D, fmt, page, dev)
+    table = i32([list(range(16))], dev)
+    kv = torch.randn((p + 8, n_kv, D), generator=gen(12)).to(BF16).to(dev)
+    paged.kv_append(pages, kv, kv.flip(0), table, i32([0], dev))
+    q = torch.randn((8, Hq, D), generator=gen(13)).to(BF16).to(dev)
+    whole = paged.attention(pages, q, table, i32([p], dev), keys_per_split=128)
+    for i in range(8):
+        one = paged.attention(pages, q[i:i + 1], table, i32([p + i], dev), keys_per_split=128)
+        assert torch.equal(one[0], whole[i])
+    two = paged.attention(pages, torch.cat([q[:3], q[4:5]]), i32([list(range(16))] * 2, dev), i32([p, p + 4], dev),
+                          cu=i32([0, 3, 4], dev), keys_per_split=128)
+    assert torch.equal(two[:3], whole[:3]) and torch.equal(two[3], whole[4])
+
+
+@pytest.mark.parametrize("fmt", ["int8", "bf16"])
+def test_pool_past_32_bits(dev, fmt):
+    """Pages whose bytes lie past 2^31 (and, in bf16, 2^32) of the pool."""
+    D, n_kv, page, n = 256, 4, 64, 33000
+    pages = paged.KVPages.alloc(n, n_kv, D, fmt, page, dev)
+    T = 100
+    kv = torch.randn((T, n_kv, D), generator=gen(14)).to(BF16).to(dev)
+    q = torch.randn((T, 16, D), generator=gen(15)).to(BF16).to(dev)
+    small = paged.KVPages.alloc(2, n_kv, D, fmt, page, dev)
+    got = []
+    for pg, tab in ((pages, [[n - 1, n - 3]]), (small, [[0, 1]])):
+        t, p0 = i32(tab, dev), i32([0], dev)
+        paged.kv_append(pg, kv, kv.flip(0), t, p0)
+        got.append([*paged.kv_read(pg, t, p0, T), paged.attention(pg, q, t, p0),
+                    paged.attention(pg, q[-1:], t, i32([T - 1], dev))])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_graph_of_the_decode_step(dev, fmt):
+    """Append, attention and read-back captured once and replayed at other positions, tables and
+    values, with eager work between the replays; two graphs on the same pages."""
+    D, Hq, n_kv, page, B, W = 256, 8, 4, 32, 3, 20
+    pages = paged.KVPages.alloc(B * W, n_kv, D, fmt, page, dev)
+    table = torch.randperm(B * W, generator=gen(16)).to(torch.int32).view(B, W).to(dev)
+    pos = i32([0, 0, 0], dev)
+    kv = torch.randn((B, 600, n_kv, D), generator=gen(17)).to(BF16).to(dev)
+    held = [300, 17, 500]
+    cu = i32(offsets(held), dev)
+    rows = torch.cat([kv[b, :n] for b, n in enumerate(held)])
+    paged.kv_append(pages, rows, rows.flip(0), table, pos, cu)
+    pos.copy_(i32(held, dev))
+    k, q = torch.empty((B, n_kv, D), dtype=BF16, device=dev), torch.empty((B, Hq, D), dtype=BF16, device=dev)
+
+    def step():
+        paged.kv_append(pages, k, k, table, pos)
+        return paged.attention(pages, q, table, pos), *paged.kv_read(pages, table, pos, B)
+
+    k.zero_()
+    q.zero_()
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step()
+        graphs.append((g, outs))
+    for i in range(6):
+        k.copy_(kv[:, 500 + i])
+        q.copy_(torch.randn((B, Hq, D), generator=gen(20 + i)).to(BF16))
+        g, outs = graphs[i % 2]
+        for o in outs:
+            o.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        pos += 1
+        if i == 2:
+            table.copy_(table.flip(1))
+            table[:, :W] = table.flip(1)
+
+
+def test_empty_calls(dev):
+    pages = paged.KVPages.alloc(2, 2, 128, "int8", 16, dev)
+    e = torch.empty((0, 2, 128), dtype=BF16, device=dev)
+    table, pos = i32([[0, 1]], dev), i32([0], dev)
+    paged.kv_append(pages, e, e, table, pos)
+    assert paged.attention(pages, e, table, pos).shape == (0, 2, 128)
+    assert paged.kv_read(pages, table, pos, 0)[0].shape == (0, 2, 128)
+    cu = i32([0, 0], dev)
+    out = torch.full((3, 2, 128), 4.0, dtype=BF16, device=dev)
+    q = torch.randn((3, 2, 128), device=dev).to(BF16)
+    paged.attention(pages, q, table, pos, cu=cu, out=out)
+    assert bool((out == 4.0).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,Hq,n_kv", [(256, 16, 4), (128, 4, 2)])
+def test_a_prompt_and_its_decode_steps(dev, fmt, D, Hq, n_kv):
+    """The operators as they are used: a prompt in chunks and single tokens after it through the input stage
+    and attention, against the same on rows kept dense."""
+    page, n = 32, 150
+    T = n + 4
+    width = Hq * 2 * D + 2 * n_kv * D
+    proj = torch.randn((T, width), generator=gen(30)).to(BF16)
+    w = (1.0 + 0.1 * torch.randn(D, generator=gen(31))).to(BF16)
+    pages = paged.KVPages.alloc(8, n_kv, D, fmt, page, dev)
+    table = [[5, 2, 7, 0, 3, -1]]
+    freqs = paged.rope_freqs(32, 1e6, dev)
+    pd, wd, td = proj.to(dev), w.to(dev), i32(table, dev)
+    outs, qs = [], []
+    for lo, hi in ((0, 64), (64, 127), (127, n), *((i, i + 1) for i in range(n, T))):
+        pos = i32([lo], dev)
+        q = paged.attn_qk_rope(pages, pd[lo:hi], wd, wd, td, pos, freqs, 1e-6)
+        gate = pd[lo:hi, :Hq * 2 * D].unflatten(1, (Hq, 2 * D))[..., D:]
+        outs.append(paged.attention(pages, q, td, pos, hi, gate=gate))
+        qs.append(q)
+    pool = ref.Pool(8, n_kv, page, D, fmt)
+    pool.k, pool.v = pages.k.cpu(), pages.v.cpu()
+    if fmt != "bf16":
+        pool.ks, pool.vs = pages.k_scale.cpu(), pages.v_scale.cpu()
+    q, gate = torch.cat(qs).cpu(), proj[:, :Hq * 2 * D].unflatten(1, (Hq, 2 * D))[..., D:]
+    want, tol = ref.attention(pool, q, table, [0], None, gate)
+    assert bool(((torch.cat(outs).cpu().double() - want).abs() <= tol).all())
+    wq, wk, wv = ref.qk_rope(proj, w, w, Hq, n_kv, D, freqs.cpu(), 1e-6, torch.arange(T))
+    assert bool(((q.double() - wq).abs() <= 2.0 ** -8 * wq.abs() + 2.0 ** -19 * wq.abs().amax(-1, keepdim=True)).all())
