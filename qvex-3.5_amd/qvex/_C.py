@@ -30,6 +30,8 @@ class KvRows(ctypes.Structure):
                 ("T", I)]
 
 
+PAGES, ROWS = ctypes.POINTER(KvPages), ctypes.POINTER(KvRows)
+
 # name -> argtypes (all return int status)
 SIGNATURES: dict[str, list] = {
     "qvex_qmv_w4g64": [P, P, P, P, P, I, I, I, P],
@@ -89,10 +91,10 @@ SIGNATURES: dict[str, list] = {
     "qvex_attention": [P, P, P, P, I, I, I, I, I, I, I, I, P, LNG, P, P, U64, P],
     "qvex_attention_decode": [P, LNG, P, P, P, I, I, I, I, I, F, P, I, P, P, I, I, I, P, P, U64, P],
     "qvex_rope_table": [I, F, I, P, P],
-    "qvex_paged_append": [P, P, P, LNG, LNG, P, LNG, LNG, P],
-    "qvex_paged_qk_rope": [P, P, P, LNG, P, P, I, I, P, F, P, P],
-    "qvex_paged_read": [P, P, P, P, I, P],
-    "qvex_paged_attention": [P, P, P, LNG, LNG, I, I, I, P, LNG, LNG, F, P, P, U64, P],
+    "qvex_paged_append": [PAGES, ROWS, P, LNG, LNG, P, LNG, LNG, P],
+    "qvex_paged_qk_rope": [PAGES, ROWS, P, LNG, P, P, I, I, P, F, P, P],
+    "qvex_paged_read": [PAGES, ROWS, P, P, I, P],
+    "qvex_paged_attention": [PAGES, ROWS, P, LNG, LNG, I, I, I, P, LNG, LNG, F, P, P, U64, P],
 }
 
 # qvex_abi_version() of the library these bindings match (8: the RoPE table of

@@ -16,20 +16,41 @@ engine/model.py:149-176), which a longer prompt moves and a shared prefix copies
 
 from __future__ import annotations
 
-import ctypes
+import functools
 
 import torch
 
 from . import _C
 from .kernels import _check
 
+_BF16, _I32, _F64 = torch.bfloat16, torch.int32, torch.float64
 FORMATS = {"bf16": (0, torch.bfloat16), "int8": (1, torch.int8), "fp8": (2, torch.float8_e4m3fn)}
 _OF_DTYPE = {t: n for n, (_, t) in FORMATS.items()}
+
+
+class _Entry:
+    """An entry point of the library, looked up at its first call (a decode step makes
+    these calls per layer: 0.5 us less than _C.call each)."""
+
+    def __init__(self, name: str):
+        self.name, self.fn = name, None
+
+    def __call__(self, *args) -> None:
+        if self.fn is None:
+            self.fn = getattr(_C.lib(), self.name)
+        rc = self.fn(*args)
+        if rc != 0:
+            raise _C.QvexError(f"{self.name} failed (status {rc}): {_C.lib().qvex_last_error().decode(errors='replace')}")
+
+
+_append, _qk_rope, _read, _attention = (_Entry("qvex_paged_" + n) for n in ("append", "qk_rope", "read", "attention"))
 
 
 class KVPages:
     """The tensors of a pool: k, v [n_pages, n_kv, page, head_dim] in bf16, int8 or
     float8_e4m3fn, and for the 8-bit types k_scale, v_scale fp32 [n_pages, n_kv, page]."""
+
+    _dev = -1       # the device's index
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
@@ -55,10 +76,9 @@ class KVPages:
             raise _C.QvexError(f"pages of {self.page} x {self.head_dim}: a power of two of 16..1024 positions, "
                                "heads of 128 or 256")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = k.device
+        self.device, self._dev = k.device, k.get_device()
         ptr = [None if t is None else t.data_ptr() for t in (k, v, k_scale, v_scale)]
         self._c = _C.KvPages(*ptr, self.n_pages, self.page, self.n_kv, self.head_dim, FORMATS[self.fmt][0])
-        self._ref = ctypes.byref(self._c)
 
     @classmethod
     def alloc(cls, n_pages: int, n_kv: int, head_dim: int, fmt: str = "int8", page: int = 64, device=None) -> "KVPages":
@@ -75,38 +95,50 @@ class KVPages:
         return [t for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None]
 
     def _stream(self) -> int:
-        if torch.cuda.current_device() != self.device.index:
+        if torch._C._cuda_getDevice() != self._dev:
             raise _C.QvexError(f"the pages are on {self.device}, the current device is "
                                f"cuda:{torch.cuda.current_device()}")
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        return torch._C._cuda_getCurrentRawStream(self._dev)
 
     def _rows(self, table, pos, T: int, cu, max_rows):
-        dev = self.device
-        B = pos.shape[0] if pos.dim() == 1 else -1
-        if pos.dtype != torch.int32 or pos.device != dev or B < 1 or not pos.is_contiguous():
-            raise _C.QvexError(f"pos must be a contiguous int32 [B] tensor on {dev} "
+        """(qvex_kv_rows, B, L, positions that a table row holds) of a call's rows."""
+        dev = self._dev
+        if pos.dtype is not _I32 or pos.get_device() != dev or pos.ndim != 1 or not pos.is_contiguous():
+            raise _C.QvexError(f"pos must be a contiguous int32 [B] tensor on {self.device} "
                                f"(got {pos.dtype} {tuple(pos.shape)} on {pos.device})")
-        if table.dtype != torch.int32 or table.device != dev or table.dim() != 2 or table.shape[0] != B \
-                or table.shape[1] < 1 or (table.stride(1) != 1 and table.shape[1] > 1):
-            raise _C.QvexError(f"table must be int32 [B = {B}, W] on {dev} with consecutive entries "
-                               f"(got {table.dtype} {tuple(table.shape)} on {table.device})")
+        B = len(pos)
+        if table.dtype is not _I32 or table.get_device() != dev or table.ndim != 2:
+            raise _C.QvexError(f"table must be int32 [B, W] on {self.device} (got {table.dtype} {tuple(table.shape)} "
+                               f"on {table.device})")
+        n, width = table.shape
+        step, one = table.stride()
+        if n != B or B < 1 or width < 1 or (one != 1 and width > 1):
+            raise _C.QvexError(f"table must be [B = {B}, W] with consecutive entries (got {tuple(table.shape)})")
         if cu is None:
             if T % B:
                 raise _C.QvexError(f"{T} rows do not divide over {B} sequences: row offsets (cu) are needed")
             L, cp = T // B, None
         else:
-            if cu.dtype != torch.int32 or cu.device != dev or cu.shape != (B + 1,) or not cu.is_contiguous():
-                raise _C.QvexError(f"cu must be a contiguous int32 [B + 1 = {B + 1}] tensor on {dev} "
+            if cu.dtype is not _I32 or cu.get_device() != dev or cu.shape != (B + 1,) or not cu.is_contiguous():
+                raise _C.QvexError(f"cu must be a contiguous int32 [B + 1 = {B + 1}] tensor on {self.device} "
                                    f"(got {cu.dtype} {tuple(cu.shape)} on {cu.device})")
             L, cp = T if max_rows is None else max(1, min(int(max_rows), T)), cu.data_ptr()
-        return ctypes.byref(_C.KvRows(table.data_ptr(), pos.data_ptr(), cp, table.stride(0), table.shape[1], B, L, T)), B, L
+        return (_C.KvRows(table.data_ptr(), pos.data_ptr(), cp, step, width, B, L, T), B, L, width * self.page)
 
-    def _heads(self, t, name: str, T: int | None, heads: int | None):
-        """A bf16 [T, heads, head_dim] view with consecutive dims on this device."""
-        if t.dtype != torch.bfloat16 or t.device != self.device or t.dim() != 3 or t.shape[2] != self.head_dim \
-                or t.stride(2) != 1 or (T is not None and t.shape[0] != T) or (heads is not None and t.shape[1] != heads):
-            raise _C.QvexError(f"{name} must be bf16 [{'T' if T is None else T}, {'H' if heads is None else heads}, "
-                               f"{self.head_dim}] on {self.device} with consecutive dims (got {t.dtype} "
+    def _heads(self, t, name: str, T: int | None = None, heads: int | None = None):
+        """(rows, heads, row stride, head stride) of a bf16 [T, heads, head_dim] view with consecutive dims."""
+        if t.dtype is _BF16 and t.get_device() == self._dev and t.ndim == 3:
+            n, h, d = t.shape
+            st, sh, one = t.stride()
+            if d == self.head_dim and one == 1 and (T is None or n == T) and (heads is None or h == heads):
+                return n, h, st, sh
+        raise _C.QvexError(f"{name} must be bf16 [{'T' if T is None else T}, {'H' if heads is None else heads}, "
+                           f"{self.head_dim}] on {self.device} with consecutive dims (got {t.dtype} "
+                           f"{tuple(t.shape)} on {t.device})")
+
+    def _out(self, t, name: str, shape, dtype):
+        if t.dtype is not dtype or t.get_device() != self._dev or t.shape != shape or not t.is_contiguous():
+            raise _C.QvexError(f"{name} must be a contiguous {dtype} {shape} tensor on {self.device} (got {t.dtype} "
                                f"{tuple(t.shape)} on {t.device})")
 
 
@@ -115,14 +147,11 @@ def kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     """Write rows k, v bf16 [T, n_kv, head_dim] (any row and head strides) at their
     sequences' next positions, quantized to the pages' format (KVCache.update,
     engine/model.py:156-170). max_rows: the most rows of a sequence, where known (speed only)."""
-    T = k.shape[0]
-    pages._heads(k, "k", None, pages.n_kv)
-    pages._heads(v, "v", T, pages.n_kv)
-    if T == 0:
-        return
-    rows, _, _ = pages._rows(table, pos, T, cu, max_rows)
-    _C.call("qvex_paged_append", pages._ref, rows, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-            v.stride(1), pages._stream())
+    T, _, kt, kh = pages._heads(k, "k", None, pages.n_kv)
+    _, _, vt, vh = pages._heads(v, "v", T, pages.n_kv)
+    if T:
+        rows = pages._rows(table, pos, T, cu, max_rows)[0]
+        _append(pages._c, rows, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, pages._stream())
 
 
 def rope_freqs(rot: int, theta: float, device) -> torch.Tensor:
@@ -139,7 +168,7 @@ def attn_qk_rope(pages: KVPages, proj: torch.Tensor, q_norm: torch.Tensor, k_nor
     2 * len(freqs) dims rotated by position * freqs (rope_freqs), k and v appended as kv_append
     does. Returns q bf16 [T, Hq, D]."""
     D = pages.head_dim
-    if proj.dtype != torch.bfloat16 or proj.device != pages.device or proj.dim() != 2 or proj.stride(1) != 1:
+    if proj.dtype is not _BF16 or proj.get_device() != pages._dev or proj.ndim != 2 or proj.stride(1) != 1:
         raise _C.QvexError(f"proj must be bf16 [T, width] on {pages.device} with consecutive columns "
                            f"(got {proj.dtype} {tuple(proj.shape)} on {proj.device})")
     T, width = proj.shape
@@ -147,24 +176,21 @@ def attn_qk_rope(pages: KVPages, proj: torch.Tensor, q_norm: torch.Tensor, k_nor
     if width % (2 * D) or Hq < 1 or Hq % pages.n_kv:
         raise _C.QvexError(f"proj rows of {width} are not [Hq x (q | gate) | k | v] with {pages.n_kv} kv heads of {D}")
     for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t.dtype != torch.bfloat16 or t.device != pages.device or t.shape != (D,) or not t.is_contiguous():
+        if t.dtype is not _BF16 or t.get_device() != pages._dev or t.shape != (D,) or not t.is_contiguous():
             raise _C.QvexError(f"{n} must be a contiguous bf16 [{D}] tensor on {pages.device}")
     rot = 0
     if freqs is not None:
-        if freqs.dtype != torch.float64 or freqs.device != pages.device or freqs.dim() != 1 or not freqs.is_contiguous():
+        if freqs.dtype is not _F64 or freqs.get_device() != pages._dev or freqs.ndim != 1 or not freqs.is_contiguous():
             raise _C.QvexError(f"freqs must be a contiguous fp64 [rot / 2] tensor on {pages.device}")
-        rot = 2 * freqs.numel()
+        rot = 2 * len(freqs)
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=proj.device)
-    elif q_out.dtype != torch.bfloat16 or q_out.device != pages.device or q_out.shape != (T, Hq, D) \
-            or not q_out.is_contiguous():
-        raise _C.QvexError(f"q_out must be a contiguous bf16 {(T, Hq, D)} tensor on {pages.device}")
-    if T == 0:
-        return q_out
-    rows, _, _ = pages._rows(table, pos, T, cu, max_rows)
-    _C.call("qvex_paged_qk_rope", pages._ref, rows, proj.data_ptr(), proj.stride(0) if T > 1 else width,
-            q_norm.data_ptr(), k_norm.data_ptr(), Hq, rot, freqs.data_ptr() if rot else None, float(eps),
-            q_out.data_ptr(), pages._stream())
+        q_out = proj.new_empty((T, Hq, D))
+    else:
+        pages._out(q_out, "q_out", (T, Hq, D), _BF16)
+    if T:
+        rows = pages._rows(table, pos, T, cu, max_rows)[0]
+        _qk_rope(pages._c, rows, proj.data_ptr(), proj.stride(0) if T > 1 else width, q_norm.data_ptr(),
+                 k_norm.data_ptr(), Hq, rot, freqs.data_ptr() if rot else None, eps, q_out.data_ptr(), pages._stream())
     return q_out
 
 
@@ -180,18 +206,18 @@ def kv_read(pages: KVPages, table: torch.Tensor, pos: torch.Tensor, T: int, cu: 
     shape = (T, pages.n_kv, pages.head_dim)
     if T < 0:
         raise _C.QvexError(f"kv_read: T={T}")
-    out = []
-    for t, n in ((k_out, "k_out"), (v_out, "v_out")):
-        if t is None:
-            t = torch.empty(shape, dtype=dtype, device=pages.device)
-        elif t.dtype != dtype or t.device != pages.device or t.shape != shape or not t.is_contiguous():
-            raise _C.QvexError(f"{n} must be a contiguous {dtype} {shape} tensor on {pages.device}")
-        out.append(t)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=pages.device)
+    else:
+        pages._out(k_out, "k_out", shape, dtype)
+    if v_out is None:
+        v_out = torch.empty_like(k_out)
+    else:
+        pages._out(v_out, "v_out", shape, dtype)
     if T:
-        rows, _, _ = pages._rows(table, pos, T, cu, max_rows)
-        _C.call("qvex_paged_read", pages._ref, rows, out[0].data_ptr(), out[1].data_ptr(),
-                int(dtype == torch.float32), pages._stream())
-    return out[0], out[1]
+        rows = pages._rows(table, pos, T, cu, max_rows)[0]
+        _read(pages._c, rows, k_out.data_ptr(), v_out.data_ptr(), int(dtype is torch.float32), pages._stream())
+    return k_out, v_out
 
 
 def attention(pages: KVPages, q: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, max_keys: int | None = None,
@@ -205,40 +231,42 @@ def attention(pages: KVPages, q: torch.Tensor, table: torch.Tensor, pos: torch.T
     rows, the table's capacity if None. keys_per_split: see qvex_paged_attention.
     workspace: any tensor of at least workspace_bytes(); one is made per call if None.
     Returns bf16 [T, Hq, D]; rows outside every sequence are left as they are in out."""
-    T, Hq = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-    pages._heads(q, "q", None, None)
+    T, Hq, qt, qh = pages._heads(q, "q")
     if Hq < 1 or Hq % pages.n_kv:
         raise _C.QvexError(f"{Hq} query heads do not share {pages.n_kv} kv heads")
     D = pages.head_dim
+    gp, gt, gh = None, 0, 0
     if gate is not None:
-        pages._heads(gate, "gate", T, Hq)
+        _, _, gt, gh = pages._heads(gate, "gate", T, Hq)
+        gp = gate.data_ptr()
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.device != pages.device or out.shape != (T, Hq, D) or not out.is_contiguous():
-        raise _C.QvexError(f"out must be a contiguous bf16 {(T, Hq, D)} tensor on {pages.device}")
+        out = q.new_empty((T, Hq, D))
+    else:
+        pages._out(out, "out", (T, Hq, D), _BF16)
     if T == 0:
         return out
-    rows, B, L = pages._rows(table, pos, T, cu, max_rows)
-    cap = table.shape[1] * pages.page
+    rows, B, L, cap = pages._rows(table, pos, T, cu, max_rows)
     mk = cap if max_keys is None else max(1, min(int(max_keys), cap))
-    need = _C.lib().qvex_paged_attention_workspace_bytes(B, L, T, Hq, pages.n_kv, D, mk, int(keys_per_split))
+    need = _workspace_bytes(B, L, T, Hq, pages.n_kv, D, mk, keys_per_split)
     have, wp = 0, None
     if need:
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        elif workspace.device != pages.device or not workspace.is_contiguous():
+            workspace = q.new_empty((need + 1) // 2)
+        elif workspace.get_device() != pages._dev or not workspace.is_contiguous():
             raise _C.QvexError(f"workspace must be a contiguous tensor on {pages.device}")
-        have, wp = workspace.numel() * workspace.element_size(), workspace.data_ptr()
-    _C.call("qvex_paged_attention", pages._ref, rows, q.data_ptr(), q.stride(0), q.stride(1), Hq, mk,
-            int(keys_per_split), None if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0),
-            0 if gate is None else gate.stride(1), D ** -0.5 if scale is None else float(scale), out.data_ptr(), wp, have,
-            pages._stream())
+        have, wp = workspace.nbytes, workspace.data_ptr()
+    _attention(pages._c, rows, q.data_ptr(), qt, qh, Hq, mk, keys_per_split, gp, gt, gh,
+               D ** -0.5 if scale is None else scale, out.data_ptr(), wp, have, pages._stream())
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(*args) -> int:
+    return _C.lib().qvex_paged_attention_workspace_bytes(*args)
 
 
 def workspace_bytes(pages: KVPages, B: int, T: int, Hq: int, max_keys: int, max_rows: int | None = None,
                     keys_per_split: int = 0) -> int:
     """Bytes of workspace that attention() takes for T rows of B sequences (0: none)."""
     L = (T // B if T % B == 0 else T) if max_rows is None else max(1, min(int(max_rows), T))
-    return int(_C.lib().qvex_paged_attention_workspace_bytes(B, L, T, Hq, pages.n_kv, pages.head_dim, int(max_keys),
-                                                             int(keys_per_split)))
+    return _workspace_bytes(B, L, T, Hq, pages.n_kv, pages.head_dim, int(max_keys), int(keys_per_split))

@@ -123,7 +123,7 @@ class _FakePages(paged.KVPages):
     def __init__(self):
         self.fmt, self.n_pages, self.n_kv, self.page, self.head_dim = "int8", 4, 2, 16, 128
         self.device = torch.device("cpu")
-        self._ref = None
+        self._c = None
 
     def _stream(self):
         raise AssertionError("a refused call reached the launch")
