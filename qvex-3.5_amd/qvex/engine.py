@@ -66,14 +66,14 @@ def prefill(model: Qwen35, ids, cache, mtp: MTPHead | None = None, mtp_cache=Non
 
 def generate(model: Qwen35, prompt_ids, params: SamplingParams, mtp: MTPHead | None = None,
              mtp_mode: str = "auto", k: int = 3, stop_ids=(), forced: list[int] | None = None,
-             max_tokens: int | None = None) -> GenerateResult:
+             max_tokens: int | None = None, kv=None) -> GenerateResult:
     """Prefill the prompt (the model runs it in 512-token chunks), hand the last
     hidden states to the MTP head, then draw tokens through decode() (MTP
     cycles replayed from a captured HIP graph) until a stop id or max_tokens
     (engine/engine.py:280-300). `forced` is shared with the
     generator: ids appended to it while iterating are emitted next, as the
     reference's reasoning budget does. A stop id counts in completion_tokens but
-    is not returned. Stats keys follow the reference's (engine/engine.py:340-357)
+    is not returned. kv: how keys and values are kept (Qwen35.make_cache). Stats keys follow the reference's (engine/engine.py:340-357)
     where they apply to this path."""
     use_mtp = mtp_policy(mtp_mode, mtp)
     ids = torch.as_tensor(prompt_ids, dtype=torch.int32).reshape(1, -1).to(model.norm.device)
@@ -89,8 +89,8 @@ def generate(model: Qwen35, prompt_ids, params: SamplingParams, mtp: MTPHead | N
     # but sized up front the captured cycle is never captured again for room
     need = ids.shape[1] + limit + 2 * k + 2
     cap = max(model.max_context, need)
-    cache = model.make_cache(max_context=cap)
-    mcache = mtp.make_cache(max_context=cap) if mtp is not None else None
+    cache = model.make_cache(max_context=cap, kv=kv)
+    mcache = mtp.make_cache(max_context=cap, kv=kv) if mtp is not None else None
     logits, last_h = prefill(model, ids, cache, mtp, mcache)
     sampler = Sampler(params, model.cfg.vocab_size)
     spec: dict = {}

@@ -29,7 +29,7 @@ from pathlib import Path
 import numpy as np
 import torch
 
-from . import _C, kernels
+from . import _C, kernels, paged
 from .kernels import _ptr, _stream
 
 QMV_MAX_ROWS = 8
@@ -686,7 +686,7 @@ class Attention:
         self.qkv_proj = QLinear.fuse([p["q_proj"], p["k_proj"], p["v_proj"]])
         self.o_proj = p["o_proj"]
         self.q_norm, self.k_norm = p["q_norm"], p["k_norm"]
-        self._ws = None
+        self._ws = self._freqs = None
 
     def _workspace(self, L, cap, kps, device):
         need = int(_C.lib().qvex_attn_workspace_bytes(L, self.n_heads, self.n_kv, self.head_dim, cap, kps))
@@ -694,7 +694,24 @@ class Attention:
             self._ws = torch.empty((need + 3) // 4, dtype=torch.float32, device=device)
         return self._ws
 
-    def __call__(self, x, cache: KVCache, resid=None, norm_w=None, eps=None):
+    def _paged(self, proj, cache: paged.PagedKVCache) -> torch.Tensor:
+        """The rows' attention over a paged cache: the input stage and the append in one launch, then the pages."""
+        L, H, D = proj.shape[0], self.n_heads, self.head_dim
+        max_keys = cache.capacity if cache.counters.graph_mode else cache.offset + L
+        if self.cfg.rotary_dim and self._freqs is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise _C.QvexError("the rotation's frequencies are made by an eager step, not inside a graph capture")
+            self._freqs = paged.rope_freqs(self.cfg.rotary_dim, self.cfg.rope_theta, proj.device)
+        pages = cache.pages
+        q = paged.attn_qk_rope(pages, proj, self.q_norm, self.k_norm, cache.table, cache.pos, self._freqs,
+                               float(self.cfg.rms_norm_eps))
+        gate = proj[:, :2 * H * D].unflatten(1, (H, 2 * D))[..., D:]
+        # one split length for the calls of a verify width: a row's bits are those of a plain step
+        o = paged.attention(pages, q, cache.table, cache.pos, max_keys, gate=gate,
+                            keys_per_split=self.decode_kps if L <= 8 else 0)
+        return o.view(L, H * D)
+
+    def __call__(self, x, cache: KVCache | paged.PagedKVCache, resid=None, norm_w=None, eps=None):
         """x [L, H] (or NormedRows); with resid the o_proj also adds the residual
         and prepares the next norm (QLinear.residual)."""
         L = x.shape[0]
@@ -706,6 +723,10 @@ class Attention:
             # replay, and decode() grows the caches and captures again)
             cache.grow(cache.offset + L)
         proj = self.qkv_proj(x)                                   # [L, H*2D + 2*Hkv*D]
+        if isinstance(cache, paged.PagedKVCache):
+            o = self._paged(proj, cache)
+            cache.offset += L
+            return self.o_proj(o) if resid is None else self.o_proj.residual(o, resid, norm_w, eps)
         pos = cache.counters.ptr(cache.index)
         # a captured call must work for every later context length: bound by capacity
         max_keys = cache.capacity if cache.counters.graph_mode else min(cache.capacity, cache.offset + L)
@@ -919,22 +940,42 @@ class Qwen35:
         self.embed, self.layers, self.norm, self.lm_head = embed, layers, norm, lm_head
         self.max_context, self.max_width = max_context, max_width
 
-    def make_cache(self, max_context: int | None = None, max_width: int | None = None):
+    def make_cache(self, max_context: int | None = None, max_width: int | None = None,
+                   kv: str | paged.PagePool | None = None):
+        """One cache per layer. kv: how the attention layers keep keys and values - None:
+        dense bf16 (KVCache); "bf16", "int8" or "fp8": in pages of that format
+        (PagedKVCache), from a pool of their own; a PagePool: in that pool's pages."""
         cfg = self.cfg
         dev = self.norm.device
         cap = max_context or self.max_context
         width = max_width or self.max_width
         counters = CacheCounters(len(self.layers), dev)
+        pool = self.kv_pool(kv, cap, sum(not l.linear for l in self.layers))
         caches = []
         for i, l in enumerate(self.layers):
             if l.linear:
                 caches.append(RecurrentCache(counters, i, conv_dim=l.mixer.conv_dim, kernel=l.mixer.K,
                                              hv=l.mixer.hv, dv=l.mixer.dv, dk=l.mixer.dk,
                                              max_width=width, device=dev, prefill_width=self.prefill_chunk))
+            elif pool is not None:
+                # of a pool that others use too, no more than was asked for
+                caches.append(paged.PagedKVCache(pool, counters, i, capacity=cap if pool is not kv else max_context or 1))
             else:
                 caches.append(KVCache(counters, i, n_kv=cfg.num_key_value_heads, head_dim=cfg.head_dim,
                                       capacity=cap, device=dev))
         return LayerCaches(caches, counters)
+
+    def kv_pool(self, kv: str | paged.PagePool | None, capacity: int, layers: int = 1) -> paged.PagePool | None:
+        """The page pool of make_cache's kv: one given, or a new one for `layers` caches of `capacity`."""
+        cfg, page = self.cfg, 64
+        if isinstance(kv, paged.PagePool) and (kv.pages.n_kv, kv.pages.head_dim) != (cfg.num_key_value_heads, cfg.head_dim):
+            raise _C.QvexError(f"the page pool holds {kv.pages.n_kv} heads of {kv.pages.head_dim}, the model has "
+                               f"{cfg.num_key_value_heads} of {cfg.head_dim}")
+        if kv is None or isinstance(kv, paged.PagePool):
+            return kv
+        size = -(-max(capacity, 1) // paged.PagedKVCache.step) * paged.PagedKVCache.step
+        return paged.PagePool(layers * (size // page), cfg.num_key_value_heads, cfg.head_dim, kv, page, self.norm.device,
+                              growable=True)
 
     def qlinears(self):
         """Every QLinear of the stack (the shared lm_head included)."""

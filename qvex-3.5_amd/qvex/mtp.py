@@ -15,7 +15,7 @@ import math
 
 import torch
 
-from . import _C, kernels
+from . import _C, kernels, paged
 from .kernels import _ptr, _stream
 from .model import (Attention, KVCache, Layer, MLP, NormedRows, QLinear, Qwen35, _rand_qlinear, add_rms_norm,
                     rms_norm)
@@ -59,10 +59,16 @@ class MTPHead:
         for q in self.qlinears():
             q.offload_mlx()
 
-    def make_cache(self, max_context: int | None = None) -> KVCache:
+    def make_cache(self, max_context: int | None = None,
+                   kv: str | paged.PagePool | None = None) -> KVCache | paged.PagedKVCache:
+        """The head's cache; kv as in Qwen35.make_cache."""
         cfg = self.model.cfg
+        cap = max_context or self.model.max_context
+        pool = self.model.kv_pool(kv, cap)
+        if pool is not None:
+            return paged.PagedKVCache(pool, capacity=cap if pool is not kv else max_context or 1)
         return KVCache(None, 0, n_kv=cfg.num_key_value_heads, head_dim=cfg.head_dim,
-                       capacity=max_context or self.model.max_context, device=self.model.norm.device)
+                       capacity=cap, device=self.model.norm.device)
 
     def __call__(self, hidden, next_ids, cache: KVCache, last_only=True, return_hidden=False, select=None,
                  argmax_out=None, defer_argmax=False, in_argmax=None, hid_sel=None, commit=None):

@@ -17,11 +17,11 @@ engine/model.py:149-176), which a longer prompt moves and a shared prefix copies
 from __future__ import annotations
 
 import functools
+import weakref
 
 import torch
 
 from . import _C
-from .kernels import _check
 
 _BF16, _I32, _F64 = torch.bfloat16, torch.int32, torch.float64
 FORMATS = {"bf16": (0, torch.bfloat16), "int8": (1, torch.int8), "fp8": (2, torch.float8_e4m3fn)}
@@ -57,8 +57,10 @@ class KVPages:
         if k.dtype not in _OF_DTYPE:
             raise _C.QvexError(f"pages must be bf16, int8 or float8_e4m3fn (got {k.dtype})")
         self.fmt = _OF_DTYPE[k.dtype]
-        _check(k, "k pages", k.dtype, 4)
-        _check(v, "v pages", k.dtype, 4)
+        for t, n in ((k, "k"), (v, "v")):
+            if t.dtype != k.dtype or t.dim() != 4 or not t.is_contiguous():
+                raise _C.QvexError(f"{n} pages must be contiguous {k.dtype} [n_pages, n_kv, page, head_dim] "
+                                   f"(got {t.dtype} {tuple(t.shape)})")
         self.n_pages, self.n_kv, self.page, self.head_dim = k.shape
         if v.shape != k.shape or v.device != k.device:
             raise _C.QvexError(f"k and v pages differ: {tuple(k.shape)} on {k.device}, {tuple(v.shape)} on {v.device}")
@@ -69,9 +71,9 @@ class KVPages:
             for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
                 if t is None:
                     raise _C.QvexError(f"{self.fmt} pages need {n}")
-                _check(t, n, torch.float32, 3)
-                if t.shape != k.shape[:3] or t.device != k.device:
-                    raise _C.QvexError(f"{n} must be {tuple(k.shape[:3])} on {k.device}")
+                if t.dtype != torch.float32 or t.shape != k.shape[:3] or t.device != k.device or not t.is_contiguous():
+                    raise _C.QvexError(f"{n} must be contiguous fp32 {tuple(k.shape[:3])} on {k.device} (got {t.dtype} "
+                                       f"{tuple(t.shape)} on {t.device})")
         if self.head_dim not in (128, 256) or self.page not in (16, 32, 64, 128, 256, 512, 1024):
             raise _C.QvexError(f"pages of {self.page} x {self.head_dim}: a power of two of 16..1024 positions, "
                                "heads of 128 or 256")
@@ -95,6 +97,8 @@ class KVPages:
         return [t for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None]
 
     def _stream(self) -> int:
+        if self._dev < 0:
+            raise _C.QvexError(f"the pages must be on a GPU (they are on {self.device})")
         if torch._C._cuda_getDevice() != self._dev:
             raise _C.QvexError(f"the pages are on {self.device}, the current device is "
                                f"cuda:{torch.cuda.current_device()}")
@@ -270,3 +274,181 @@ def workspace_bytes(pages: KVPages, B: int, T: int, Hq: int, max_keys: int, max_
     """Bytes of workspace that attention() takes for T rows of B sequences (0: none)."""
     L = (T // B if T % B == 0 else T) if max_rows is None else max(1, min(int(max_rows), T))
     return _workspace_bytes(B, L, T, Hq, pages.n_kv, pages.head_dim, int(max_keys), int(keys_per_split))
+
+
+# ---------------------------------------------------------------- pages handed to sequences
+
+class PagePool:
+    """A pool's pages and who holds them: ``take`` gives free pages, ``share`` adds a
+    holder (a prefix that two sequences have in common), ``give`` ends a hold. A page
+    with several holders is only read. growable: ``take`` enlarges the pool when
+    it runs out, as KVCache.grow does (the tensors move; refused while a captured
+    cycle drives a cache of the pool); otherwise running out raises.
+
+    Pages change hands in the order of the calls: caches of one pool are used on one
+    stream, or the caller orders their streams."""
+
+    def __init__(self, n_pages: int, n_kv: int, head_dim: int, fmt: str = "int8", page: int = 64, device=None,
+                 growable: bool = False):
+        self.pages = KVPages.alloc(n_pages, n_kv, head_dim, fmt, page, device)
+        self.growable = growable
+        self.holders = [0] * n_pages
+        self.free = list(range(n_pages - 1, -1, -1))
+        self.users: weakref.WeakSet = weakref.WeakSet()
+
+    @property
+    def page(self) -> int:
+        return self.pages.page
+
+    def take(self, n: int) -> list[int]:
+        if n > len(self.free):
+            if not self.growable:
+                raise _C.QvexError(f"the page pool has {len(self.free)} free pages of {self.pages.n_pages}, {n} are needed")
+            self.grow(max(n - len(self.free), self.pages.n_pages // 2))
+        got = [self.free.pop() for _ in range(n)]
+        for j in got:
+            self.holders[j] = 1
+        return got
+
+    def share(self, ids) -> None:
+        for j in ids:
+            self.holders[j] += 1
+
+    def give(self, ids) -> None:
+        for j in ids:
+            self.holders[j] -= 1
+            if self.holders[j] == 0:
+                self.free.append(j)
+
+    def copy(self, src: int, dst: int) -> None:
+        for t in self.pages.tensors():
+            t[dst].copy_(t[src])
+
+    def grow(self, n: int) -> None:
+        """n more pages: larger tensors that start with the old ones' pages."""
+        if any(c.counters.graph_mode for c in self.users):
+            raise _C.QvexError("a captured cycle drives a cache of this page pool; release() it before the pool grows")
+        old = self.pages
+        new = KVPages.alloc(old.n_pages + n, old.n_kv, old.head_dim, old.fmt, old.page, old.device)
+        for a, b in zip(new.tensors(), old.tensors()):
+            a[:old.n_pages].copy_(b)
+        self.pages = new
+        self.holders += [0] * n
+        self.free = list(range(new.n_pages - 1, old.n_pages - 1, -1)) + self.free
+
+
+class PagedKVCache:
+    """One sequence's keys and values of one layer in a pool's pages, with KVCache's
+    interface (offset, rollback, grow, clone, keys, values; engine/model.py:149-176).
+    Growing adds pages to its table and moves no key; a clone shares the whole
+    pages of the prefix and copies the one that the next key goes to.
+
+    The page of position ``offset`` and all behind it have this cache as their only holder
+    (clone and rollback see to it), so an append never writes a shared page."""
+
+    step = 256
+
+    def __init__(self, pool: PagePool, counters=None, index: int = 0, *, capacity: int = 0):
+        if counters is None:
+            from .model import CacheCounters
+            counters, index = CacheCounters(1, pool.pages.device), 0
+        self.pool, self.counters, self.index = pool, counters, index
+        self.ids: list[int] = []
+        self.table = torch.full((1, 1), -1, dtype=torch.int32, device=pool.pages.device)
+        self.pos = counters.dev[index:index + 1]
+        pool.users.add(self)
+        self._extend(max(capacity, 1))
+
+    def __del__(self):
+        if getattr(self, "ids", None):
+            self.pool.give(self.ids)
+
+    @property
+    def pages(self) -> KVPages:
+        return self.pool.pages
+
+    @property
+    def capacity(self) -> int:
+        return len(self.ids) * self.pool.page
+
+    @property
+    def offset(self) -> int:
+        return self.counters.get(self.index)
+
+    @offset.setter
+    def offset(self, v: int) -> None:
+        if v < self.offset:
+            self.counters._check_host_edit()
+            self._own(max(v, 0))
+        self.counters.set(self.index, v)
+
+    def rollback(self, n=1):
+        self.offset -= n     # entries past offset are overwritten by the next append
+
+    def state(self):
+        return self.pages.tensors()
+
+    def _extend(self, min_capacity: int) -> None:
+        size = -(-min_capacity // self.step) * self.step
+        self.ids += self.pool.take(-(-size // self.pool.page) - len(self.ids))
+        self._upload()
+
+    def _upload(self) -> None:
+        if self.table.shape[1] < len(self.ids):
+            self.table = torch.full((1, len(self.ids)), -1, dtype=torch.int32, device=self.table.device)
+        self.table[0, :len(self.ids)].copy_(torch.tensor(self.ids, dtype=torch.int32))
+
+    def _own(self, at: int) -> None:
+        """The pages from position `at` on become this cache's alone."""
+        first, changed = at // self.pool.page, False
+        for x in range(first, len(self.ids)):
+            j = self.ids[x]
+            if self.pool.holders[j] > 1:
+                self.ids[x] = self.pool.take(1)[0]
+                if x == first and at % self.pool.page:
+                    self.pool.copy(j, self.ids[x])
+                self.pool.give([j])
+                changed = True
+        if changed:
+            self._upload()
+
+    def grow(self, min_capacity: int) -> bool:
+        """Pages for at least min_capacity positions, in steps of 256 (a HIP graph
+        captured on the cache must be captured again). Returns whether any were added."""
+        self.counters._check_host_edit()
+        if min_capacity <= self.capacity:
+            return False
+        self._extend(min_capacity)
+        return True
+
+    def clone(self, counters=None) -> "PagedKVCache":
+        """A cache of the same keys that shares the prefix's whole pages; counters:
+        the cloned table it indexes (a new one-entry table for a standalone cache).
+        Its capacity is what the prefix needs, and grows."""
+        c = PagedKVCache.__new__(PagedKVCache)
+        c.pool = self.pool
+        c.counters = counters if counters is not None else self.counters.clone()
+        c.index, c.ids = self.index, []
+        c.pos = c.counters.dev[c.index:c.index + 1]
+        n = self.offset // self.pool.page
+        size = -(-(self.offset + 1) // self.step) * self.step
+        fresh = self.pool.take(-(-size // self.pool.page) - n)
+        if self.offset % self.pool.page:
+            self.pool.copy(self.ids[n], fresh[0])
+        self.pool.share(self.ids[:n])
+        c.ids = self.ids[:n] + fresh
+        c.table = torch.full((1, len(c.ids)), -1, dtype=torch.int32, device=self.table.device)
+        c._upload()
+        self.pool.users.add(c)
+        return c
+
+    def _rows(self) -> torch.Tensor:
+        return torch.zeros(1, dtype=torch.int32, device=self.table.device)
+
+    def keys(self) -> torch.Tensor:
+        """K as bf16 [n_kv, capacity, D] (a copy)."""
+        return kv_read(self.pages, self.table, self._rows(), self.capacity)[0].transpose(0, 1).contiguous()
+
+    def values(self) -> torch.Tensor:
+        """V as bf16 [n_kv, capacity, D] (a copy)."""
+        return kv_read(self.pages, self.table, self._rows(), self.capacity)[1].transpose(0, 1).contiguous()

@@ -107,14 +107,21 @@ def test_workspace_bytes():
         assert kps == 0 or sizes == sorted(sizes)
 
 
-def test_front_end_refuses_host_tensors():
-    k = torch.zeros((2, 2, 16, 128), dtype=torch.int8)
-    with pytest.raises(_C.QvexError, match="GPU tensor"):
-        paged.KVPages(k, k, torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16)))
-    with pytest.raises(_C.QvexError, match="bf16, int8"):
-        paged.KVPages(k.float(), k.float())
+def test_front_end_refuses_bad_pools_and_host_memory():
+    k, s = torch.zeros((2, 2, 16, 128), dtype=torch.int8), torch.zeros((2, 2, 16))
+    for args, match in (((k.float(), k.float()), "bf16, int8"), ((k, k), "need k_scale"), ((k, k[:1], s, s), "differ"),
+                        ((k, k.to(BF16), s, s), "v pages"), ((k, k, s, s.double()), "v_scale"),
+                        ((k, k, s, s[:1]), "v_scale"), ((k.to(BF16), k.to(BF16), s), "no scales"),
+                        ((k[..., :64].contiguous(), k[..., :64].contiguous(), s, s), "heads of 128 or 256"),
+                        ((k[:, :, :8].contiguous(), k[:, :, :8].contiguous(), s[..., :8].contiguous(),
+                          s[..., :8].contiguous()), "power of two")):
+        with pytest.raises(_C.QvexError, match=match):
+            paged.KVPages(*args)
     with pytest.raises(_C.QvexError, match="unknown KV format"):
         paged.KVPages.alloc(2, 2, 128, "int4")
+    x, t, p = torch.zeros((1, 2, 128), dtype=BF16), torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(_C.QvexError, match="must be on a GPU"):
+        paged.kv_append(paged.KVPages(k, k, s, s), x, x, t, p)
 
 
 class _FakePages(paged.KVPages):
@@ -176,3 +183,113 @@ def test_front_end_refuses_rows_without_offsets():
         paged.kv_read(_FakePages(), a["table"], a["pos"], 6, dtype=torch.float16)
     with pytest.raises(_C.QvexError, match="out must"):
         paged.attention(_FakePages(), a["x"], a["table"], a["pos"], out=torch.zeros((6, 2, 128)))
+
+
+# ---------------------------------------------------------------- pages handed to sequences
+
+def fill(pool):
+    """Every page's bytes name the page."""
+    for j in range(pool.pages.n_pages):
+        for x in pool.pages.tensors():
+            x[j] = j % 100 + 1
+
+
+def test_pool_takes_shares_and_gives():
+    pool = paged.PagePool(4, 2, 128, "int8", 16, "cpu")
+    a = pool.take(3)
+    assert sorted(a) == [0, 1, 2] and pool.free == [3]
+    pool.share(a[:1])
+    pool.give(a)
+    assert sorted(pool.free) == [1, 2, 3] and pool.holders == [1, 0, 0, 0]
+    with pytest.raises(_C.QvexError, match="3 free pages of 4, 5"):
+        pool.take(5)
+    assert sorted(pool.free) == [1, 2, 3]
+    pool.give(a[:1])
+    assert len(pool.free) == 4
+
+
+@pytest.mark.parametrize("fmt", ["int8", "bf16"])
+def test_pool_grows_and_keeps_its_pages(fmt):
+    pool = paged.PagePool(2, 2, 128, fmt, 16, "cpu", growable=True)
+    fill(pool)
+    old = [x.clone() for x in pool.pages.tensors()]
+    got = pool.take(5)
+    assert len(set(got)) == 5 and pool.pages.n_pages >= 5
+    for a, b in zip(pool.pages.tensors(), old):
+        assert torch.equal(a[:2], b)
+
+
+def test_cache_grows_without_moving_and_returns_its_pages():
+    pool = paged.PagePool(40, 2, 128, "fp8", 16, "cpu")
+    c = paged.PagedKVCache(pool, capacity=100)
+    assert c.capacity == 256 and len(pool.free) == 24
+    first = c.table[0, :16].clone()
+    c.offset = 250
+    assert not c.grow(256) and c.grow(257) and c.capacity == 512
+    assert torch.equal(c.table[0, :16], first) and c.table[0].tolist() == c.ids
+    with pytest.raises(_C.QvexError, match="free pages"):
+        c.grow(1000)
+    c.counters.graph_mode = True
+    with pytest.raises(_C.QvexError, match="captured cycle"):
+        c.grow(600)
+    with pytest.raises(_C.QvexError, match="captured cycle"):
+        c.rollback(1)
+    c.counters.graph_mode = False
+    del c
+    assert len(pool.free) == 40 and not any(pool.holders)
+
+
+def test_pool_does_not_move_under_a_captured_cycle():
+    pool = paged.PagePool(16, 2, 128, "int8", 16, "cpu", growable=True)
+    a = paged.PagedKVCache(pool, capacity=256)
+    a.counters.graph_mode = True
+    with pytest.raises(_C.QvexError, match="captured cycle drives a cache of this page pool"):
+        paged.PagedKVCache(pool, capacity=256)
+    a.counters.graph_mode = False
+    paged.PagedKVCache(pool, capacity=256)
+
+
+@pytest.mark.parametrize("at", [0, 1, 15, 16, 40, 255, 256, 300])
+def test_clone_shares_the_prefix_and_an_append_never_writes_a_shared_page(at):
+    pool = paged.PagePool(200, 2, 128, "int8", 16, "cpu")
+    fill(pool)
+    a = paged.PagedKVCache(pool, capacity=512)
+    a.offset = at
+    b = a.clone()
+    n = at // 16
+    assert b.offset == at and b.ids[:n] == a.ids[:n] and not set(b.ids[n:]) & set(a.ids)
+    assert b.capacity > at and b.table[0].tolist() == b.ids
+    if at % 16:      # the page that the next key goes to has the prefix's bytes
+        for x in pool.pages.tensors():
+            assert torch.equal(x[b.ids[n]], x[a.ids[n]])
+    for c in (a, b):
+        assert all(pool.holders[j] == 1 for j in c.ids[c.offset // 16:])
+    # rolled back into the shared part, a cache takes pages of its own, with what they held
+    if at > 20:
+        held = list(a.ids)
+        a.rollback(20)
+        m = a.offset // 16
+        assert a.ids[:m] == held[:m] and all(pool.holders[j] == 1 for j in a.ids[m:])
+        assert b.ids[:n] == held[:n] and not set(a.ids[m:]) & set(b.ids)
+        assert a.table[0, :len(a.ids)].tolist() == a.ids
+        if a.offset % 16:
+            for x in pool.pages.tensors():
+                assert torch.equal(x[a.ids[m]], x[held[m]])
+    c = b.clone()
+    assert pool.holders == [sum(j in x.ids for x in (a, b, c)) for j in range(200)]
+    del a, b, c
+    assert len(pool.free) == 200 and not any(pool.holders)
+
+
+def test_clone_of_layer_caches_shares_one_table_of_counters():
+    from qvex.model import CacheCounters, LayerCaches
+    pool = paged.PagePool(64, 2, 128, "int8", 64, "cpu")
+    counters = CacheCounters(2, "cpu")
+    caches = LayerCaches([paged.PagedKVCache(pool, counters, i, capacity=256) for i in range(2)], counters)
+    for c in caches:
+        c.offset = 130
+    twin = caches.clone()
+    assert twin[0].counters is twin[1].counters is twin.counters and twin.counters is not counters
+    twin[0].offset = 131
+    assert caches[0].offset == 130 and twin[1].offset == 130
+    assert twin[0].pos.data_ptr() == twin.counters.ptr(0) and caches[1].pos.data_ptr() == counters.ptr(1)

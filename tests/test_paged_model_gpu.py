@@ -1,0 +1,197 @@
+"""The model on paged caches (Qwen35.make_cache(kv=...)): an attention layer against float64 over
+what its pages hold, decode() on the captured cycle, growth, shared prefixes, generate()."""
+
+import pytest
+import torch
+
+import paged_ref as ref
+from qvex import _C, paged
+from qvex.engine import generate, prefill
+from qvex.model import Config, random_model
+from qvex.mtp import random_mtp
+from qvex.sampler import Sampler, SamplingParams
+from qvex.speculative import decode
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["bf16", "int8", "fp8"]
+
+
+@pytest.fixture(scope="module")
+def tiny(dev):
+    model = random_model(Config.tiny(layers=4, vocab=2048), seed=5, device=dev, max_context=512)
+    return model, random_mtp(model, seed=6)
+
+
+def ids_of(n, vocab, seed=0):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return torch.randint(0, vocab, (1, n), generator=g, dtype=torch.int32)
+
+
+class _Keep:
+    """An o_proj that keeps what it was given."""
+
+    def __call__(self, o):
+        self.o = o
+        return o
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [[1, 4, 8], [70, 9, 1, 130]])
+def test_attention_layer_over_pages(dev, tiny, fmt, rows):
+    """Chunks and single rows through Attention on a paged cache, against float64 attention over the
+    values that the pages stand for (q from the input stage run again on a pool of its own)."""
+    model, _ = tiny
+    cfg, layer = model.cfg, next(l.mixer for l in model.layers if not l.linear)
+    H, n_kv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+    cache = model.make_cache(max_context=256, kv=fmt)[-1]
+    keep, o_proj = _Keep(), layer.o_proj
+    layer.o_proj = keep
+    try:
+        at = 0
+        for n in rows:
+            g = torch.Generator()
+            g.manual_seed(n)
+            x = torch.randn((n, cfg.hidden_size), generator=g).to(torch.bfloat16).to(dev)
+            proj = layer.qkv_proj(x)
+            cache.counters.sync()
+            layer(x, cache)
+            assert cache.offset == at + n
+            pool = ref.Pool(cache.pages.n_pages, n_kv, cache.pages.page, D, fmt)
+            pool.k, pool.v = cache.pages.k.cpu(), cache.pages.v.cpu()
+            if fmt != "bf16":
+                pool.ks, pool.vs = cache.pages.k_scale.cpu(), cache.pages.v_scale.cpu()
+            scratch = paged.KVPages.alloc(cache.pages.n_pages, n_kv, D, fmt, cache.pages.page, dev)
+            q = paged.attn_qk_rope(scratch, proj, layer.q_norm, layer.k_norm, cache.table,
+                                   torch.tensor([at], dtype=torch.int32, device=dev),
+                                   paged.rope_freqs(cfg.rotary_dim, cfg.rope_theta, dev), cfg.rms_norm_eps)
+            gate = proj.cpu()[:, :2 * H * D].reshape(n, H, 2 * D)[..., D:]
+            want, tol = ref.attention(pool, q.cpu(), cache.table.tolist(), [at], None, gate)
+            assert bool(((keep.o.cpu().double().view(n, H, D) - want).abs() <= tol).all())
+            at += n
+    finally:
+        layer.o_proj = o_proj
+    k = cache.keys()
+    assert k.shape == (n_kv, cache.capacity, D) and bool((k[:, at:] == 0).all()) and bool((k[:, :at] != 0).any())
+
+
+def run(model, mtp, ids, kv, n, graph=True, k=3, temperature=0.0, use_mtp=True, cap=None):
+    cache = model.make_cache(max_context=cap, kv=kv)
+    mc = mtp.make_cache(max_context=cap, kv=kv)
+    logits, last = prefill(model, ids, cache, mtp, mc)
+    smp = Sampler(SamplingParams(temperature=temperature, top_k=20 if temperature else 0,
+                                 top_p=0.8 if temperature else 1.0, seed=3), model.cfg.vocab_size)
+    st: dict = {}
+    gen = decode(model, smp, cache, logits[0, -1], last, mtp, mc, lambda: use_mtp, st, k=k, graph=graph)
+    out = [next(gen) for _ in range(n)]
+    gen.close()
+    return out, st, cache
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_decode_is_the_same_captured_eager_and_plain(tiny, fmt):
+    """On pages as on dense caches: the captured cycle emits the eager one's tokens (sampled too), and greedy
+    speculation emits plain greedy decoding's."""
+    model, mtp = tiny
+    ids = ids_of(77, model.cfg.vocab_size)
+    a, st, _ = run(model, mtp, ids, fmt, 24)
+    assert st["graph_cycles"] > 0
+    assert a == run(model, mtp, ids, fmt, 24, graph=False)[0]
+    assert a == run(model, mtp, ids, fmt, 24, use_mtp=False)[0]
+    s = run(model, mtp, ids, fmt, 24, temperature=0.9)[0]
+    assert s == run(model, mtp, ids, fmt, 24, graph=False, temperature=0.9)[0]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_decode_past_the_capacity_grows(tiny, fmt):
+    """A prompt that ends 3 positions before the capacity: the caches grow, in the captured path too."""
+    model, mtp = tiny
+    ids = ids_of(253, model.cfg.vocab_size, seed=1)
+    a, _, cache = run(model, mtp, ids, fmt, 20, cap=256)
+    assert cache[-1].capacity > 256
+    assert a == run(model, mtp, ids, fmt, 20, cap=1024)[0]
+    assert a == run(model, mtp, ids, fmt, 20, cap=256, graph=False)[0]
+
+
+def test_two_branches_of_a_shared_prefix(dev, tiny):
+    """Sequences that share a prefix's pages go on as if each had its own, also after a rollback into it."""
+    model, _ = tiny
+    V = model.cfg.vocab_size
+    pool = paged.PagePool(200, model.cfg.num_key_value_heads, model.cfg.head_dim, "int8", 16, dev)
+
+    def more(cache, ids):
+        return model(ids, cache, last_only=False).clone()
+
+    def fresh(*parts):
+        cache = model.make_cache(max_context=256, kv="int8")
+        out = None
+        for p in parts:
+            out = more(cache, p)
+        return out
+
+    prefix, x, y = ids_of(61, V, 2), ids_of(7, V, 3), ids_of(5, V, 4)
+    a = model.make_cache(max_context=256, kv=pool)
+    more(a, prefix)
+    used = 200 - len(pool.free)
+    b = a.clone()
+    assert 200 - len(pool.free) < 2 * used        # the whole pages of the prefix are not copied
+    assert torch.equal(more(b, y), fresh(prefix, y)) and torch.equal(more(a, x), fresh(prefix, x))
+    z = ids_of(3, V, 5)
+    assert torch.equal(more(b, z), fresh(prefix, y, z)) and torch.equal(more(a, z), fresh(prefix, x, z))
+    del a, b
+    assert len(pool.free) == 200
+
+
+def test_rollback_into_a_shared_page(dev, tiny):
+    """KV pages only (a verify of rejected drafts after a clone): the twin's keys stay."""
+    model, _ = tiny
+    cfg = model.cfg
+    pool = paged.PagePool(40, cfg.num_key_value_heads, cfg.head_dim, "int8", 16, dev)
+    a = paged.PagedKVCache(pool, capacity=64)
+    g = torch.Generator()
+    g.manual_seed(9)
+    kv = torch.randn((40, cfg.num_key_value_heads, cfg.head_dim), generator=g).to(torch.bfloat16).to(dev)
+
+    def put(c, rows):
+        c.counters.sync()
+        paged.kv_append(c.pages, rows, rows, c.table, c.pos)
+        c.offset += rows.shape[0]
+
+    put(a, kv)
+    b = a.clone()
+    kept = b.keys()[:, :40].clone()
+    a.rollback(20)
+    put(a, -kv[:20])
+    assert torch.equal(b.keys()[:, :40], kept) and torch.equal(b.values()[:, :40], kept)
+    k = a.keys()
+    assert torch.equal(k[:, :20], kept[:, :20]) and torch.equal(k[:, 20:40], -kept[:, :20])
+
+
+def test_generate_on_pages(tiny):
+    model, mtp = tiny
+    params = SamplingParams(temperature=0.0, top_k=0, top_p=1.0, max_tokens=20)
+    ids = ids_of(40, model.cfg.vocab_size, 6)
+    for fmt in FORMATS:
+        on = generate(model, ids, params, mtp, "on", kv=fmt)
+        off = generate(model, ids, params, mtp, "off", kv=fmt)
+        assert on.tokens == off.tokens and len(on.tokens) == 20 and on.stats["mtp_cycles"] > 0
+    pool = paged.PagePool(64, model.cfg.num_key_value_heads, model.cfg.head_dim, "int8", 64, model.norm.device)
+    assert generate(model, ids, params, mtp, "on", kv=pool).tokens == generate(model, ids, params, mtp, "on", kv="int8").tokens
+    assert len(pool.free) == 64
+    with pytest.raises(_C.QvexError, match="unknown KV format"):
+        generate(model, ids, params, mtp, "on", kv="int4")
+    with pytest.raises(_C.QvexError, match="page pool holds"):
+        model.make_cache(kv=paged.PagePool(4, 1, 128, "int8", 64, model.norm.device))
+
+
+def test_bf16_pages_and_dense_caches_agree(tiny):
+    """The same prompt, chunk and steps: logits within two bf16 steps of the largest."""
+    model, _ = tiny
+    V = model.cfg.vocab_size
+    outs = []
+    for kv in (None, "bf16"):
+        cache = model.make_cache(max_context=512, kv=kv)
+        outs.append([model(ids_of(n, V, n), cache, last_only=False).float() for n in (130, 40, 4, 1)])
+    for a, b in zip(*outs):
+        assert float((a - b).abs().max()) <= 2 * 2.0 ** -7 * float(a.abs().max())
