@@ -59,8 +59,8 @@ inline int kv_check(const char* fn, const qvex_kv_pages* p, const qvex_kv_rows* 
   QVEX_CHECK_ARG(p->D == 128 || p->D == 256, "%s: D=%d (128 or 256 supported)", fn, p->D);
   QVEX_CHECK_ARG(p->page >= 16 && p->page <= 1024 && (p->page & (p->page - 1)) == 0,
                  "%s: page=%d must be a power of two, 16..1024", fn, p->page);
-  QVEX_CHECK_ARG(p->n_pages >= 1 && p->Hkv >= 1 && p->Hkv <= 1024, "%s: n_pages=%d Hkv=%d (1..1024)", fn, p->n_pages,
-                 p->Hkv);
+  QVEX_CHECK_ARG(p->n_pages >= 1 && p->Hkv >= 1 && p->Hkv <= 1024 && (int64_t)p->n_pages * p->Hkv * p->page < 1LL << 31,
+                 "%s: n_pages=%d Hkv=%d (1..1024; page * n_pages * Hkv below 2^31)", fn, p->n_pages, p->Hkv);
   QVEX_CHECK_ARG(p->k && p->v && qvex_aligned(p->k, 16) && qvex_aligned(p->v, 16),
                  "%s: the pages of K and V must be 16-byte aligned, not null", fn);
   QVEX_CHECK_ARG(p->format == QVEX_KV_BF16 || (p->k_scales && p->v_scales && qvex_aligned(p->k_scales, 16) &&

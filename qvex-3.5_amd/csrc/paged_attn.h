@@ -1,0 +1,125 @@
+// What the two forms of paged attention share (paged_attn.hip: calls of few rows;
+// paged_chunk.hip: prompt chunks): their arguments, the steps from codes to
+// bf16, the records of a split, the epilogue.
+#pragma once
+#include "paged.h"
+
+namespace {
+
+typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pa_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
+typedef float pa_f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int PA_ROWS = 16;            // rows of a tile of few rows
+constexpr int PA_STEP = 128;           // keys that splits are multiples of
+constexpr float PA_NONE = -3.0e38f;    // m before any visible key
+constexpr float PA_SLACK = 8.0f;       // m moves when a score (base 2) passes it by more: P up to 256
+
+struct PaArgs {
+  KvPages c;
+  KvRows r;
+  const uint16_t* q;
+  long q_token, q_head;
+  const uint16_t* gate;
+  long g_token, g_head;
+  uint16_t* out;
+  float* ws;                           // O [T * Hq][nsplit][D], then (m, l) [T * Hq][nsplit]
+  int Hq, kps, nsplit, vec;
+  float c2;                            // scale * log2(e): scores in base 2
+};
+
+__device__ __forceinline__ pa_bf16x8 as_pa8(const u32x4 v) { return __builtin_bit_cast(pa_bf16x8, v); }
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((pa_f32x2{lo, hi}), pa_bf16x2));
+}
+__device__ __forceinline__ float2* pa_ml(const PaArgs& a, int D) {
+  return reinterpret_cast<float2*>(a.ws + (size_t)a.r.T * a.Hq * a.nsplit * D);
+}
+
+// A uniform word of the block table: a scalar load.
+__device__ __forceinline__ int pa_page(const int32_t* t, int i) {
+  return ((const __attribute__((address_space(4))) int32_t*)t)[i];
+}
+
+__device__ __forceinline__ u32x4 pa_load8(const uint16_t* p, int vec) {
+  if (vec) return load16(p);
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  return w;
+}
+
+// Codes e .. e + 7 of eight bytes as bf16.
+template <int FMT>
+__device__ __forceinline__ u32x4 codes8(uint32_t lo, uint32_t hi) {
+  u32x4 o;
+  if constexpr (FMT == QVEX_KV_FP8) {
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  } else {
+    o[0] = pa_pack((float)(int8_t)lo, (float)(int8_t)(lo >> 8));
+    o[1] = pa_pack((float)(int8_t)(lo >> 16), (float)(int8_t)(lo >> 24));
+    o[2] = pa_pack((float)(int8_t)hi, (float)(int8_t)(hi >> 8));
+    o[3] = pa_pack((float)(int8_t)(hi >> 16), (float)(int8_t)(hi >> 24));
+  }
+  return o;
+}
+
+// The A operands of tiles 2 t and 2 t + 1: values 2 t and 2 t + 1 of each of eight keys' runs v.
+template <int FMT, int VW>
+__device__ __forceinline__ void gather2(const uint32_t (&v)[8][VW], int t, u32x4& a0, u32x4& a1) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (FMT == QVEX_KV_BF16) {
+      a0[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x05040100u);
+      a1[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x07060302u);
+    } else {
+      const uint32_t x = v[2 * i][t >> 1], y = v[2 * i + 1][t >> 1];
+      if constexpr (FMT == QVEX_KV_FP8) {
+        const uint32_t w = __builtin_amdgcn_perm(y, x, t & 1 ? 0x07030602u : 0x05010400u);
+        a0[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+        a1[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+      } else {
+        const int s = t & 1 ? 16 : 0;
+        a0[i] = pa_pack((float)(int8_t)(x >> s), (float)(int8_t)(y >> s));
+        a1[i] = pa_pack((float)(int8_t)(x >> (s + 8)), (float)(int8_t)(y >> (s + 8)));
+      }
+    }
+  }
+}
+
+// The word with 0 for every infinity and NaN.
+template <int FMT>
+__device__ __forceinline__ uint32_t tame(uint32_t w) {
+  if constexpr (FMT == QVEX_KV_BF16)
+    return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+  uint32_t o = w;
+  if constexpr (FMT == QVEX_KV_FP8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((w >> (8 * i) & 0x7fu) == 0x7fu) o &= ~(0xffu << (8 * i));
+  }
+  return o;
+}
+
+__device__ __forceinline__ void pa_gate_store(const PaArgs& a, int t, int h, int d, int D, const float (&o)[4]) {
+  uint16_t* op = a.out + ((size_t)t * a.Hq + h) * D + d;
+  float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+  if (a.gate) {
+    const uint16_t* gp = a.gate + t * a.g_token + h * a.g_head + d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = 1.0f / (1.0f + expf(-bf16_to_f32(gp[i])));
+  }
+  *reinterpret_cast<u32x2*>(op) = u32x2{pack_bf16x2(o[0] * g[0], o[1] * g[1]), pack_bf16x2(o[2] * g[2], o[3] * g[3])};
+}
+
+}  // namespace
+
+namespace qvex {
+// Launches the chunk form on checked arguments: `tiles` blocks of rows for the longest sequence.
+constexpr int PA_CHUNK_ROWS = 128;
+void paged_chunk_attention(const void* args, int format, int D, int tiles, int B, void* stream);
+}  // namespace qvex

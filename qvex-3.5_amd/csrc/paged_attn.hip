@@ -16,118 +16,9 @@
 // So K, V and P never leave their lanes, and a lane owns one q row. Codes are exact in
 // bf16: K's scale multiplies the score, V's the weight. P goes into the second product
 // as two bf16 terms (16 bits of it), so the output's own rounding is the one that shows.
-#include "paged.h"
+#include "paged_attn.h"
 
 namespace {
-
-typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 pa_bf16x2 __attribute__((ext_vector_type(2)));
-typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
-typedef float pa_f32x2 __attribute__((ext_vector_type(2)));
-
-constexpr int PA_ROWS = 16;            // rows of a tile
-constexpr int PA_STEP = 128;           // keys of a block's step: 32 per wave
-constexpr float PA_NONE = -3.0e38f;    // m before any visible key
-constexpr float PA_SLACK = 8.0f;       // m moves when a score (base 2) passes it by more: P up to 256
-
-struct PaArgs {
-  KvPages c;
-  KvRows r;
-  const uint16_t* q;
-  long q_token, q_head;
-  const uint16_t* gate;
-  long g_token, g_head;
-  uint16_t* out;
-  float* ws;                           // O [T * Hq][nsplit][D], then (m, l) [T * Hq][nsplit]
-  int Hq, kps, nsplit, vec;
-  float c2;                            // scale * log2(e): scores in base 2
-};
-
-__device__ __forceinline__ pa_bf16x8 as_pa8(const u32x4 v) { return __builtin_bit_cast(pa_bf16x8, v); }
-__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((pa_f32x2{lo, hi}), pa_bf16x2));
-}
-__device__ __forceinline__ float2* pa_ml(const PaArgs& a, int D) {
-  return reinterpret_cast<float2*>(a.ws + (size_t)a.r.T * a.Hq * a.nsplit * D);
-}
-
-// A uniform word of the block table: a scalar load.
-__device__ __forceinline__ int pa_page(const int32_t* t, int i) {
-  return ((const __attribute__((address_space(4))) int32_t*)t)[i];
-}
-
-__device__ __forceinline__ u32x4 pa_load8(const uint16_t* p, int vec) {
-  if (vec) return load16(p);
-  u32x4 w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-  return w;
-}
-
-// Codes e .. e + 7 of eight bytes as bf16.
-template <int FMT>
-__device__ __forceinline__ u32x4 codes8(uint32_t lo, uint32_t hi) {
-  u32x4 o;
-  if constexpr (FMT == QVEX_KV_FP8) {
-    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
-    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
-    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
-    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
-  } else {
-    o[0] = pa_pack((float)(int8_t)lo, (float)(int8_t)(lo >> 8));
-    o[1] = pa_pack((float)(int8_t)(lo >> 16), (float)(int8_t)(lo >> 24));
-    o[2] = pa_pack((float)(int8_t)hi, (float)(int8_t)(hi >> 8));
-    o[3] = pa_pack((float)(int8_t)(hi >> 16), (float)(int8_t)(hi >> 24));
-  }
-  return o;
-}
-
-// The A operands of tiles 2 t and 2 t + 1: values 2 t and 2 t + 1 of each of eight keys' runs v.
-template <int FMT, int VW>
-__device__ __forceinline__ void gather2(const uint32_t (&v)[8][VW], int t, u32x4& a0, u32x4& a1) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (FMT == QVEX_KV_BF16) {
-      a0[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x05040100u);
-      a1[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x07060302u);
-    } else {
-      const uint32_t x = v[2 * i][t >> 1], y = v[2 * i + 1][t >> 1];
-      if constexpr (FMT == QVEX_KV_FP8) {
-        const uint32_t w = __builtin_amdgcn_perm(y, x, t & 1 ? 0x07030602u : 0x05010400u);
-        a0[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-        a1[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
-      } else {
-        const int s = t & 1 ? 16 : 0;
-        a0[i] = pa_pack((float)(int8_t)(x >> s), (float)(int8_t)(y >> s));
-        a1[i] = pa_pack((float)(int8_t)(x >> (s + 8)), (float)(int8_t)(y >> (s + 8)));
-      }
-    }
-  }
-}
-
-// Whether a word of V holds an infinity or a NaN.
-template <int FMT>
-__device__ __forceinline__ bool wild(uint32_t w) {
-  if constexpr (FMT == QVEX_KV_BF16) return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-  if constexpr (FMT == QVEX_KV_FP8) {
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) any |= (w >> (8 * i) & 0x7fu) == 0x7fu;
-    return any;
-  }
-  return false;
-}
-
-__device__ __forceinline__ void pa_gate_store(const PaArgs& a, int t, int h, int d, int D, const float (&o)[4]) {
-  uint16_t* op = a.out + ((size_t)t * a.Hq + h) * D + d;
-  float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-  if (a.gate) {
-    const uint16_t* gp = a.gate + t * a.g_token + h * a.g_head + d;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = 1.0f / (1.0f + expf(-bf16_to_f32(gp[i])));
-  }
-  *reinterpret_cast<u32x2*>(op) = u32x2{pack_bf16x2(o[0] * g[0], o[1] * g[1]), pack_bf16x2(o[2] * g[2], o[3] * g[3])};
-}
 
 // One block per (kv head, 16-row tile, sequence, split): its 4 waves take 32 keys each of every
 // 128, alone until their (m, l, O) are merged in LDS.
@@ -292,7 +183,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 #pragma unroll
           for (int u = 0; u < VW; ++u) {
             if (!live) vr[e][u] = 0;
-            any |= key > s.pos + i_lo && wild<FMT>(vr[e][u]);
+            any |= key > s.pos + i_lo && tame<FMT>(vr[e][u]) != vr[e][u];
           }
         }
         apart = __any(any);
@@ -391,6 +282,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
   }
 }
 
+// A call of more than 8 rows per sequence takes the chunk form (paged_chunk.hip) if a sequence's
+// rows of a kv head fill half a block and (query, key) pairs * D are worth its start and end,
+// 8 us against 3. us, this form | that one, int8, 16 query and 4 kv heads of 256 (pairs = T * Hq *
+// max_keys): 64 positions at 1000 keys (1.1M) 23 | 24, at 4000 (4.2M) 34 | 33, 512 at 0 (4.2M) 30 | 27,
+// 8 x 64 at 1000 (8.7M) 47 | 39, at 4000 (33M) 111 | 72, 512 at 4000 (37M) 119 | 75; of 128, 4 and 2
+// heads: 512 at 4000 (9.2M) 33 | 30, 12 x 100 at 1000 (5.3M) 24 | 24, 8 x 200 at 4000 (27M) 67 | 50.
+constexpr long PA_CHUNK_MIN = 64;
+constexpr double PA_CHUNK_WORK = 5e6 * 256;
+
 // A row's records merged; D / 4 lanes hold the row, four dims each, eight records requested
 // at a time. WIDE: a block per row, whose groups of lanes take every 256 / (D / 4)-th record and
 // are then merged in their order: few rows of many records are otherwise a chain of round trips
@@ -468,6 +368,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
 }
 
 struct PaPlan {
+  bool chunk;                          // paged_chunk.hip's form
   int tiles, kps, nsplit;              // row tiles of the longest sequence; keys per split; splits
   uint64_t bytes;
 };
@@ -476,11 +377,13 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
   if (B < 1 || L < 1 || T < 0 || Hkv < 1 || Hq < Hkv || Hq % Hkv || (D != 128 && D != 256) || max_keys < 1 ||
       max_keys > KV_LIMIT || kps < 0 || kps % PA_STEP)
     return false;
-  const long GQ = Hq / Hkv, tiles = (std::min(L, std::max(T, 1)) * GQ + PA_ROWS - 1) / PA_ROWS;
-  const long steps = (max_keys + PA_STEP - 1) / PA_STEP;
+  const long GQ = Hq / Hkv, most = std::min(L, std::max(T, 1)) * GQ;
+  p->chunk = L > 8 && most >= PA_CHUNK_MIN && (double)T * Hq * max_keys * D >= PA_CHUNK_WORK;
+  const int per = p->chunk ? qvex::PA_CHUNK_ROWS : PA_ROWS;
+  const long tiles = (most + per - 1) / per, steps = (max_keys + PA_STEP - 1) / PA_STEP;
   if (kps == 0) {
-    const long blocks = std::min(B * tiles, T * GQ / PA_ROWS + B) * Hkv;
-    const long n = std::min(std::max(1024 / std::max(blocks, 1L), 1L), steps);
+    const long blocks = std::min(B * tiles, T * GQ / per + B) * Hkv, want = p->chunk ? 256 : 1024;
+    const long n = std::min(std::max(want / std::max(blocks, 1L), 1L), steps);
     kps = (int)((steps + n - 1) / n) * PA_STEP;
   }
   p->tiles = (int)std::min<long>(tiles, 1 << 20);
@@ -516,6 +419,7 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
                  "%s: Hq=%d Hkv=%d max_keys=%d keys_per_split=%d (a multiple of 128, or 0)", fn, Hq, a.c.Hkv, max_keys,
                  keys_per_split);
   QVEX_CHECK_ARG(p.nsplit <= 65535, "%s: grid too large", fn);
+  QVEX_CHECK_ARG(scale >= 0.0f && scale < INFINITY, "%s: scale=%g must be finite, not negative", fn, (double)scale);
   if (a.r.T == 0) return QVEX_OK;
   QVEX_CHECK_ARG(q && out && qvex_aligned(q, 2) && qvex_aligned(out, 16) && qvex_aligned(gate, 2),
                  "%s: null or misaligned q, gate or out (out 16-byte aligned)", fn);
@@ -534,7 +438,7 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
   a.kps = p.kps;
   a.nsplit = p.nsplit;
   a.vec = (q_token % 8 | q_head % 8) == 0 && qvex_aligned(q, 16);
-  a.c2 = scale * 1.44269504088896340736f;
+  a.c2 = fmaxf(scale * 1.44269504088896340736f, 1e-37f);       // a masked score stays -inf at a scale of 0 too
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid(a.c.Hkv * p.tiles, B, p.nsplit);
   const int f = pages->format;
@@ -544,7 +448,8 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
                            : (f == QVEX_KV_BF16   ? &launch_attn<QVEX_KV_BF16, 128>
                               : f == QVEX_KV_INT8 ? &launch_attn<QVEX_KV_INT8, 128>
                                                   : &launch_attn<QVEX_KV_FP8, 128>);
-  go(grid, st, a);
+  if (p.chunk) qvex::paged_chunk_attention(&a, f, D, p.tiles, B, stream);
+  else go(grid, st, a);
   QVEX_CHECK_LAUNCH(fn);
   if (p.nsplit > 1) {
     // wide by the rows of a sequence alone, so that calls of up to 8 give a row the same bits

@@ -88,14 +88,15 @@ def read(pool, table, pos, T, cu=None, fill=0.0):
     return k, v
 
 
-def attention(pool, q, table, pos, cu=None, gate=None, scale=None, fill=0.0):
+def attention(pool, q, table, pos, cu=None, gate=None, scale=None, fill=0.0, terms=2):
     """(out, tol): the rows' attention in float64 and how far a correct kernel may be from it.
 
     The kernel's errors, u = 2^-24: a score is a sum of D fp32 products (D u of the sum
     of magnitudes, times 3 for its scale, its conversion to base 2 and the argument's
     subtraction), which moves its weight by as much, relatively, and the sum of
     the weights too; exp2 is good to 2 u; a weight goes into the product as two bf16 terms
-    (2^-16 of it); sums over n weights n u. The output is rounded to bf16 (2^-8)."""
+    (2^-16 of it), or, in calls of more than 8 rows per sequence (terms=1), as one (2^-8
+    of it); sums over n weights n u. The output is rounded to bf16 (2^-8)."""
     T, Hq, D = q.shape
     scale = D ** -0.5 if scale is None else scale
     out = torch.full((T, Hq, D), fill, dtype=torch.float64)
@@ -127,7 +128,7 @@ def attention(pool, q, table, pos, cu=None, gate=None, scale=None, fill=0.0):
                 o = w @ V[live, g]
                 mag = (K[live, g].abs() @ qq.abs()) * abs(scale)
                 delta = 3 * (D + 8) * u * float(mag.max()) + (2 + len(w)) * u
-                a = (w.abs() @ V[live, g].abs()) * (2.0 ** -16 + 2 * delta)
+                a = (w.abs() @ V[live, g].abs()) * (2.0 ** (-16 if terms == 2 else -8) + 2 * delta)
                 if gate is not None:
                     sg = torch.sigmoid(gate[t, h].double())
                     o, a = o * sg, a * sg + o.abs() * sg * 8 * u

@@ -216,10 +216,13 @@ def test_qk_rope_values_are_appended_as_append_does(dev):
 # ---------------------------------------------------------------- attention
 
 def check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, *, gate=False, scale=None, seed=8, poison=True, kps=0,
-                    max_keys=None, max_rows=None, pad=0, fill_gain=1.0, edit=None):
+                    max_keys=None, max_rows=None, pad=0, fill_gain=1.0, edit=None, wide=False):
+    """wide: a table of many unused entries, whose capacity as the bound of the keys makes a call of many
+    rows a large one, so that it takes the form of prompt chunks."""
     g = gen(seed)
     T = sum(lens) + pad
-    table, n_pages = layout(lens, pos, page, seed + 1)
+    extra = -(-1_300_000_000 // (T * Hq * D * page)) if wide else 1
+    table, n_pages = layout(lens, pos, page, seed + 1, extra_width=extra)
     pool = ref.Pool(n_pages, n_kv, page, D, fmt)
     if poison:          # what no sequence holds is no data
         if fmt == "bf16":
@@ -243,7 +246,8 @@ def check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, *, gate=False, scale
     pages = gpu_pool(pool, dev)
     paged.attention(pages, q.to(dev), i32(tab, dev), i32(pos, dev), max_keys, i32(cu, dev), max_rows,
                     gd[..., D:] if gate else None, scale, out, keys_per_split=kps)
-    want, tol = ref.attention(pool, q, tab, pos, cu, gt[..., D:] if gate else None, scale, fill=9.0)
+    want, tol = ref.attention(pool, q, tab, pos, cu, gt[..., D:] if gate else None, scale, fill=9.0,
+                              terms=2 if min(max_rows or T, T) <= 8 else 1)
     got = out.cpu().double()
     assert torch.equal(got.isfinite(), want.isfinite())
     fin = want.isfinite()
@@ -264,6 +268,17 @@ def test_attention(dev, fmt, D, Hq, n_kv, page, lens, pos):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kps", [0, 1 << 20, 256])
+@pytest.mark.parametrize("D,Hq,n_kv,page,lens,pos", [
+    (256, 16, 4, 64, [20], [0]), (256, 8, 4, 16, [33], [190]), (256, 16, 1, 256, [40], [300]), (128, 4, 2, 32, [130, 1, 65], [0, 200, 63]),
+    (128, 4, 4, 16, [70, 0, 9], [5, 40, 127]), (256, 4, 4, 64, [129], [64]), (128, 6, 2, 1024, [50], [1000]),
+])
+def test_attention_of_prompt_chunks(dev, fmt, kps, D, Hq, n_kv, page, lens, pos):
+    """One split (a split length past every key) and many."""
+    check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, kps=kps, gate=kps == 0, wide=True)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("kps,max_keys", [(128, None), (256, 1200), (0, 1), (128, 130), (1152, None)])
 def test_attention_splits(dev, fmt, kps, max_keys):
     """Any split, and a bound on the keys that is too small."""
@@ -274,6 +289,10 @@ def test_attention_splits(dev, fmt, kps, max_keys):
 def test_attention_gate_scale_padding(dev, fmt):
     check_attention(dev, fmt, 256, 8, 4, 32, [3, 12], [77, 0], gate=True, scale=0.02, pad=4)
     check_attention(dev, fmt, 128, 4, 2, 16, [3, 40], [77, 0], max_rows=1, fill_gain=30.0)
+    check_attention(dev, fmt, 256, 8, 4, 32, [3, 50], [77, 0], gate=True, scale=0.02, pad=4, wide=True)
+    check_attention(dev, fmt, 128, 4, 2, 16, [3, 140], [77, 0], max_rows=33, fill_gain=30.0, wide=True)
+    check_attention(dev, fmt, 128, 4, 2, 16, [3, 40], [77, 9], scale=0.0, wide=True)
+    check_attention(dev, fmt, 128, 4, 2, 16, [3], [77], scale=0.0)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -286,13 +305,18 @@ def test_attention_rows_that_see_nothing(dev, fmt, long):
         tab[0][0] = -1                          # the first page of sequence 0
         tab[2] = [99] * len(tab[2])
 
-    got, _ = check_attention(dev, fmt, 128, 4, 2, 16, [n, n, n], [5, -4, 20], edit=edit)
+    if long:
+        check_attention(dev, fmt, 128, 4, 2, 16, [n, n, n], [5, -4, 20], edit=edit, wide=True, kps=1 << 20)
+        check_attention(dev, fmt, 128, 4, 2, 16, [n, n, n], [-100, -4, -69], edit=edit, wide=True, kps=1 << 20)
+    got, _ = check_attention(dev, fmt, 128, 4, 2, 16, [n, n, n], [5, -4, 20], edit=edit, wide=long)
     assert bool((got[n:n + 4] == 0).all()) and bool((got[2 * n:3 * n] == 0).all()) and bool((got[:min(n, 11)] == 0).all())
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("D,Hq,n_kv,n", [(256, 16, 4, 4), (128, 4, 2, 40), (256, 4, 2, 90), (128, 16, 1, 3)])
-def test_attention_nan_and_inf_stay_with_the_rows_that_see_them(dev, fmt, D, Hq, n_kv, n):
+@pytest.mark.parametrize("D,Hq,n_kv,n", [(256, 16, 4, 4), (128, 4, 2, 40), (256, 4, 2, 90), (128, 16, 1, 3), (128, 2, 2, 200),
+                                         (256, 16, 4, 30)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_nan_and_inf_stay_with_the_rows_that_see_them(dev, fmt, D, Hq, n_kv, n, wide):
     """A key or value that is not a number, seen by later rows only; a query that is not one."""
     pos = 61
 
@@ -308,7 +332,7 @@ def test_attention_nan_and_inf_stay_with_the_rows_that_see_them(dev, fmt, D, Hq,
         pool.put(pool.slot(tab[0], pos + n - 1), k2, v)
         q[1, 0, 5] = math.nan
 
-    _, want = check_attention(dev, fmt, D, Hq, n_kv, 16, [n], [pos], edit=edit)
+    _, want = check_attention(dev, fmt, D, Hq, n_kv, 16, [n], [pos], edit=edit, wide=wide)
     assert bool(want[0].isfinite().all()) and not bool(want[n - 1].isfinite().all())
 
 
@@ -363,6 +387,7 @@ def test_pool_past_32_bits(dev, fmt):
         t, p0 = i32(tab, dev), i32([0], dev)
         paged.kv_append(pg, kv, kv.flip(0), t, p0)
         got.append([*paged.kv_read(pg, t, p0, T), paged.attention(pg, q, t, p0),
+                    paged.attention(pg, q, torch.cat([t, torch.full((1, 100), -1, dtype=torch.int32, device=dev)], 1), p0),
                     paged.attention(pg, q[-1:], t, i32([T - 1], dev))])
     for a, b in zip(*got):
         assert torch.equal(a, b)
@@ -454,7 +479,7 @@ def test_a_prompt_and_its_decode_steps(dev, fmt, D, Hq, n_kv):
     if fmt != "bf16":
         pool.ks, pool.vs = pages.k_scale.cpu(), pages.v_scale.cpu()
     q, gate = torch.cat(qs).cpu(), proj[:, :Hq * 2 * D].unflatten(1, (Hq, 2 * D))[..., D:]
-    want, tol = ref.attention(pool, q, table, [0], None, gate)
+    want, tol = ref.attention(pool, q, table, [0], None, gate, terms=1)
     assert bool(((torch.cat(outs).cpu().double() - want).abs() <= tol).all())
     wq, wk, wv = ref.qk_rope(proj, w, w, Hq, n_kv, D, freqs.cpu(), 1e-6, torch.arange(T))
     assert bool(((q.double() - wq).abs() <= 2.0 ** -8 * wq.abs() + 2.0 ** -19 * wq.abs().amax(-1, keepdim=True)).all())
