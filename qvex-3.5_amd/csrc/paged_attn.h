@@ -91,6 +91,32 @@ __device__ __forceinline__ void gather2(const uint32_t (&v)[8][VW], int t, u32x4
   }
 }
 
+// Lane i of each 16-lane row, in every lane of that row.
+template <int I>
+__device__ __forceinline__ float row_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + I, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float row_lane_of(float v, int i) {   // i a constant after unrolling
+  switch (i) {
+    case 0: return row_lane<0>(v);
+    case 1: return row_lane<1>(v);
+    case 2: return row_lane<2>(v);
+    case 3: return row_lane<3>(v);
+    case 4: return row_lane<4>(v);
+    case 5: return row_lane<5>(v);
+    case 6: return row_lane<6>(v);
+    case 7: return row_lane<7>(v);
+    case 8: return row_lane<8>(v);
+    case 9: return row_lane<9>(v);
+    case 10: return row_lane<10>(v);
+    case 11: return row_lane<11>(v);
+    case 12: return row_lane<12>(v);
+    case 13: return row_lane<13>(v);
+    case 14: return row_lane<14>(v);
+    default: return row_lane<15>(v);
+  }
+}
+
 // The word with 0 for every infinity and NaN.
 template <int FMT>
 __device__ __forceinline__ uint32_t tame(uint32_t w) {
@@ -105,16 +131,26 @@ __device__ __forceinline__ uint32_t tame(uint32_t w) {
   return o;
 }
 
-__device__ __forceinline__ void pa_gate_store(const PaArgs& a, int t, int h, int d, int D, const float (&o)[4]) {
-  uint16_t* op = a.out + ((size_t)t * a.Hq + h) * D + d;
-  float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-  if (a.gate) {
+// sigmoid(gate) of four dims of a row (1 without a gate), asked for where it is made, and the row's
+// epilogue.
+struct PaGate {
+  uint16_t g[4];
+  __device__ __forceinline__ PaGate(const PaArgs& a, int t, int h, int d) {
+    if (!a.gate) return;
     const uint16_t* gp = a.gate + t * a.g_token + h * a.g_head + d;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = 1.0f / (1.0f + expf(-bf16_to_f32(gp[i])));
+    for (int i = 0; i < 4; ++i) g[i] = gp[i];
   }
-  *reinterpret_cast<u32x2*>(op) = u32x2{pack_bf16x2(o[0] * g[0], o[1] * g[1]), pack_bf16x2(o[2] * g[2], o[3] * g[3])};
-}
+  __device__ __forceinline__ void store(const PaArgs& a, int t, int h, int d, int D, const float (&o)[4]) const {
+    float f[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (a.gate) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = 1.0f / (1.0f + expf(-bf16_to_f32(g[i])));
+    }
+    *reinterpret_cast<u32x2*>(a.out + ((size_t)t * a.Hq + h) * D + d) =
+        u32x2{pack_bf16x2(o[0] * f[0], o[1] * f[1]), pack_bf16x2(o[2] * f[2], o[3] * f[3])};
+  }
+};
 
 }  // namespace
 

@@ -21,13 +21,16 @@
 namespace {
 
 // One block per (kv head, 16-row tile, sequence, split): its 4 waves take 32 keys each of every
-// 128, alone until their (m, l, O) are merged in LDS.
-template <int FMT, int D>
+// 128, alone until their (m, l, O) are merged in LDS. PIPE (splits of several steps): the next
+// step's K is asked for once the scores have this one's, its V behind the second product (us, 8
+// sequences of up to 8192 keys in int8, one split each: 124 -> 95); a split of one step has no next.
+template <int FMT, int D, bool PIPE>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 #pragma clang fp contract(off)
   constexpr int EB = kv_bytes(FMT), KS = D / 32, KU = D * EB / 64, E = D / 16, VW = E * EB / 4, ROW = D * EB;
   __shared__ __align__(16) float obuf[4][PA_ROWS][D + 4];
   __shared__ float2 mlbuf[4][PA_ROWS];
+  __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int li = lane & 15, lg = lane >> 4;
   const int b = blockIdx.y, split = blockIdx.z, kh = blockIdx.x % a.c.Hkv, GQ = a.Hq / a.c.Hkv;
@@ -51,6 +54,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
     const int k_hi = split == a.nsplit - 1 ? keys : min(k_lo + a.kps, keys);
     if (k_lo >= k_hi) continue;                                   // uniform; the merge does not read it
 
+    if (FMT != QVEX_KV_INT8) {
+      if (threadIdx.x == 0) odd = 0;
+      __syncthreads();
+    }
     u32x4 qa[KS];
     const uint16_t* qp = a.q + (s.first + i) * a.q_token + (kh * GQ + g) * a.q_head;
 #pragma unroll
@@ -61,7 +68,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 
     u32x4 kr[2][KU];
     uint32_t vr[8][VW];
-    float ksc[8], vsc[8];
+    float ksc = 0.0f, vsc = 0.0f;                                 // lane e of 16: of key 8 lg + e
     bool ok0 = true, ok1 = true;                                  // of the block's two 16-key halves
     long at0 = 0, at1 = 0;
     auto locate = [&](int kb, int p0, int p1) __attribute__((always_inline)) {
@@ -78,9 +85,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 #pragma unroll
         for (int u = 0; u < KU; ++u) kr[h][u] = load16(p + 4 * h * ROW + 64 * u);
       if constexpr (EB == 1) {
-        const float* sp = a.c.ks + (lg >> 1 ? at1 : at0) + 8 * (lg & 1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ksc[e] = sp[e];
+        ksc = a.c.ks[(lg >> 1 ? at1 : at0) + 8 * (lg & 1) + (li & 7)];
       }
     };
     auto load_v = [&]() __attribute__((always_inline)) {
@@ -101,11 +106,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
           }
         }
       }
-      if constexpr (EB == 1) {
-        const float* sp = a.c.vs + at;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) vsc[e] = sp[e];
-      }
+      if constexpr (EB == 1) vsc = a.c.vs[at + (li & 7)];
     };
 
     const pa_f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -114,13 +115,27 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 #pragma unroll
     for (int n = 0; n < E; ++n) o[n] = zero;
 
-    int p0 = first0, p1 = first1;
-    for (int kb = k_lo + 32 * wave; kb < k_hi; kb += PA_STEP) {
+    int kb = k_lo + 32 * wave, p0 = first0, p1 = first1;
+    if (PIPE && kb < k_hi) {
       locate(kb, p0, p1);
-      p0 = page_at(kb + PA_STEP);                                 // the next step's
+      p0 = page_at(kb + PA_STEP);
       p1 = page_at(kb + PA_STEP + 16);
       load_k();
       load_v();
+    }
+    if (PIPE) {
+#pragma unroll
+      for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(qa[st]));   // Q waited for here, not in the loop with all of V
+    }
+    for (; kb < k_hi; kb += PA_STEP) {
+      if (!PIPE) {
+        locate(kb, p0, p1);
+        p0 = page_at(kb + PA_STEP);                               // the next step's
+        p1 = page_at(kb + PA_STEP + 16);
+        load_k();
+        load_v();
+      }
+      const bool here0 = ok0, here1 = ok1;                        // of this step
       pa_f32x4 sc[2] = {zero, zero};
 #pragma unroll
       for (int st = 0; st < KS; ++st)
@@ -131,21 +146,35 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
           else ka = codes8<FMT>(kr[h][st >> 1][2 * (st & 1)], kr[h][st >> 1][2 * (st & 1) + 1]);
           sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(ka), as_pa8(qa[st]), sc[h], 0, 0, 0);
         }
+      if (PIPE) __builtin_amdgcn_sched_barrier(0);                // V is not touched (nor waited for) before its product
       float t[8], top = -INFINITY;
       uint32_t vis = 0xff;                                        // of the lane's keys 8 lg ..
-      const bool edge = kb + 32 > min(s.pos + i_lo + 1, k_hi) || !ok0 || !ok1;   // uniform
+      const bool edge = kb + 32 > min(s.pos + i_lo + 1, k_hi) || !here0 || !here1;   // uniform
       if (edge) {
         vis = 0;
-        if (lg >> 1 ? ok1 : ok0)
+        if (lg >> 1 ? here1 : here0)
 #pragma unroll
           for (int e = 0; e < 8; ++e) vis |= (kb + 8 * lg + e <= min(rlim, k_hi - 1) ? 1u : 0u) << e;
       }
+      const float kf = EB == 1 ? ksc * a.c2 : a.c2;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        t[e] = sc[e >> 2][e & 3] * a.c2;
-        if constexpr (EB == 1) t[e] *= ksc[e];
+        t[e] = sc[e >> 2][e & 3] * (EB == 1 ? row_lane_of(kf, e) : kf);
         if (edge && !(vis >> e & 1)) t[e] = -INFINITY;
         top = fmaxf(top, t[e]);
+      }
+      if (PIPE) {
+        // behind the last step of the wave this one again, so that the loads need no branch (a branch would have
+        // their registers copied, and so waited for)
+        const bool more = kb + PA_STEP < k_hi;
+        const int kn = more ? kb + PA_STEP : kb;
+        if (more) {
+          locate(kn, p0, p1);
+          p0 = page_at(kn + PA_STEP);
+          p1 = page_at(kn + PA_STEP + 16);
+        }
+        load_k();
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (__any(top - m > PA_SLACK)) {
         float x = fmaxf(top, __shfl_xor(top, 16, 64));
@@ -164,59 +193,33 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
       for (int e = 0; e < 8; ++e) {
         t[e] = __builtin_amdgcn_exp2f(t[e] - m);
         l += t[e];
-        if constexpr (EB == 1) t[e] = edge && !(vis >> e & 1) ? 0.0f : t[e] * vsc[e];
+        if constexpr (EB == 1) {
+          const float w = t[e] * row_lane_of(vsc, e);             // by all lanes: a lane that is off gives nothing
+          t[e] = edge && !(vis >> e & 1) ? 0.0f : w;
+        }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         p[e] = pa_pack(t[2 * e], t[2 * e + 1]);
         p_lo[e] = pa_pack(t[2 * e] - bf16_lo(p[e]), t[2 * e + 1] - bf16_hi(p[e]));
       }
-      bool apart = false;
       if (edge && FMT != QVEX_KV_INT8) {
-        // what no row of the tile sees is not data, and 0 times a NaN or an infinity
-        // is none: keys past the last row's (and pages that are not there) become 0
+        // what no row of the tile sees is not data, and 0 times a NaN or an infinity is none: keys past the last
+        // row's (and pages that are not there) become 0. So does a NaN or an infinity that some rows do
+        // not see: the rows that do are marked at the end
         bool any = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int key = kb + 8 * lg + e;
-          const bool live = key < k_hi && (lg >> 1 ? ok1 : ok0);
+          const bool live = key < k_hi && (lg >> 1 ? here1 : here0);
 #pragma unroll
           for (int u = 0; u < VW; ++u) {
-            if (!live) vr[e][u] = 0;
-            any |= key > s.pos + i_lo && tame<FMT>(vr[e][u]) != vr[e][u];
+            const uint32_t w = live ? vr[e][u] : 0, w1 = key > s.pos + i_lo ? tame<FMT>(w) : w;
+            any |= w1 != w;
+            vr[e][u] = w1;
           }
         }
-        apart = __any(any);
-      }
-      if (apart) {
-        // some rows see a NaN or an infinity that others of the tile do not: the keys that
-        // not every row sees are added one by one, and left out of the product
-#pragma unroll 1
-        for (int kg = 0; kg < 4; ++kg) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int key = kb + 8 * kg + e;
-            if (key <= s.pos + i_lo || key >= k_hi || !(kg >> 1 ? ok1 : ok0)) continue;   // uniform
-            const float w = __shfl(t[e], 16 * kg + li, 64);
-            const uint8_t* p1 = a.c.v + ((kg >> 1 ? at1 : at0) + 8 * (kg & 1) + e) * ROW;
-            if (key <= rlim)
-#pragma unroll
-              for (int n = 0; n < E; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int d = E * (4 * lg + j) + n;
-                  float x;
-                  if constexpr (EB == 2) x = bf16_to_f32(reinterpret_cast<const uint16_t*>(p1)[d]);
-                  else x = __builtin_amdgcn_cvt_f32_fp8((int)p1[d], 0);
-                  o[n][j] = fmaf(w, x, o[n][j]);
-                }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int u = 0; u < VW; ++u)
-            if (kb + 8 * lg + e > s.pos + i_lo) vr[e][u] = 0;
+        if (any) odd = 1;
       }
 #pragma unroll
       for (int n = 0; n < E; n += 2) {
@@ -227,6 +230,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
         o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(a1), as_pa8(p), o[n + 1], 0, 0, 0);
         o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_pa8(a1), as_pa8(p_lo), o[n + 1], 0, 0, 0);
       }
+      if (PIPE) load_v();
     }
 
     // the waves' sums, merged in the order of the waves
@@ -261,11 +265,25 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
         acc[2] = fmaf(ov.z, f, acc[2]);
         acc[3] = fmaf(ov.w, f, acc[3]);
       }
+      if (FMT != QVEX_KV_INT8 && odd) {
+        for (int key = max(k_lo, s.pos + i_lo + 1); key < k_hi && key <= s.pos + rw / GQ; ++key) {
+          const int pg = table[key >> a.c.shift];
+          if (pg < 0 || pg >= a.c.n_pages) continue;
+          const uint8_t* pv = a.c.v + ((((long)pg * a.c.Hkv + kh) << a.c.shift) + (key & mask)) * ROW + d * EB;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            bool bad;
+            if constexpr (EB == 2) bad = (reinterpret_cast<const uint16_t*>(pv)[e] & 0x7f80u) == 0x7f80u;
+            else bad = (pv[e] & 0x7fu) == 0x7fu;
+            if (bad) acc[e] = __uint_as_float(0x7fc00000u);
+          }
+        }
+      }
       if (a.nsplit == 1) {
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] *= inv;
-        pa_gate_store(a, tok, head, d, D, acc);
+        PaGate(a, tok, head, d).store(a, tok, head, d, D, acc);
       } else {
         const size_t rec = ((size_t)tok * a.Hq + head) * a.nsplit + split;
         *reinterpret_cast<float4*>(a.ws + rec * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -294,7 +312,7 @@ constexpr double PA_CHUNK_WORK = 5e6 * 256;
 // A row's records merged; D / 4 lanes hold the row, four dims each, eight records requested
 // at a time. WIDE: a block per row, whose groups of lanes take every 256 / (D / 4)-th record and
 // are then merged in their order: few rows of many records are otherwise a chain of round trips
-// (us, 16 rows of 33 records 10.4 -> 5.2, 64 of 55 17.0 -> 7.1; many rows of few records need the lanes).
+// (us, 16 rows of 33 records 10.4 -> 4.1, 64 of 28 -> 5.0; many rows of few records need the lanes).
 template <int D, bool WIDE>
 __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
 #pragma clang fp contract(off)
@@ -308,21 +326,27 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
   const int each = WIDE ? 1 : PER;
   for (long w = (long)blockIdx.x * each + (WIDE ? 0 : sub); w < rows; w += (long)gridDim.x * each) {
     const int i = (int)(w / a.Hq), h = (int)(w - (long)i * a.Hq), tok = s.first + i;
-    const int keys = min(s.pos + i + 1, cap);
-    const int act = keys <= 0 ? 0 : min((keys - 1) / a.kps + 1, a.nsplit);
     const size_t rec = ((size_t)tok * a.Hq + h) * a.nsplit;
     const float2* mls = pa_ml(a, D) + rec;
     const float* os = a.ws + rec * D + d;
     float m = PA_NONE, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = WIDE ? sub : 0; s0 < act; s0 += BATCH * STEP) {
-      float2 ml[BATCH];
-      float4 ov[BATCH];
+    // the first records are asked for before the position says how many there are (what the others hold is dropped)
+    float2 ml[BATCH];
+    float4 ov[BATCH];
+    auto ask = [&](int s0, int n) __attribute__((always_inline)) {
 #pragma unroll
       for (int x = 0; x < BATCH; ++x) {
-        const int at = min(s0 + x * STEP, act - 1);
+        const int at = min(s0 + x * STEP, n - 1);
         ml[x] = mls[at];
         ov[x] = *reinterpret_cast<const float4*>(os + (size_t)at * D);
       }
+    };
+    ask(WIDE ? sub : 0, a.nsplit);
+    const PaGate gate(a, tok, h, d);
+    const int keys = min(s.pos + i + 1, cap);
+    const int act = keys <= 0 ? 0 : min((keys - 1) / a.kps + 1, a.nsplit);
+    for (int s0 = WIDE ? sub : 0; s0 < act; s0 += BATCH * STEP) {
+      if (s0 >= BATCH * STEP) ask(s0, act);
 #pragma unroll
       for (int x = 0; x < BATCH; ++x) {
         if (s0 + x * STEP >= act) break;
@@ -361,7 +385,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] *= inv;
-      pa_gate_store(a, tok, h, d, D, o);
+      gate.store(a, tok, h, d, D, o);
     }
     if constexpr (WIDE) __syncthreads();
   }
@@ -382,9 +406,14 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
   const int per = p->chunk ? qvex::PA_CHUNK_ROWS : PA_ROWS;
   const long tiles = (most + per - 1) / per, steps = (max_keys + PA_STEP - 1) / PA_STEP;
   if (kps == 0) {
-    const long blocks = std::min(B * tiles, T * GQ / per + B) * Hkv, want = p->chunk ? 256 : 1024;
-    const long n = std::min(std::max(want / std::max(blocks, 1L), 1L), steps);
-    kps = (int)((steps + n - 1) / n) * PA_STEP;
+    // as many splits as give each CU a block (us, int8, 256-dim heads, blocks of one split | n splits: 16
+    // x 2000 keys (64 blocks) 28 | 4: 18 | 16: 22; 8 x 4 rows at 4096 (32) 54 | 8: 21 | 33: 30; 64 x 4600 (256) 112
+    // | 2: 112 | 36: 154), of two steps at least where a tile is more than half full (its
+    // records cost more than the second step: 4 rows at 7001 keys 16 | 14)
+    const long blocks = std::max(std::min(B * tiles, T * GQ / per + B) * Hkv, 1L);
+    const long want = p->chunk || L <= 8 ? 256 : 768;             // many row tiles of unequal lengths
+    const long n = std::min(std::max(want / blocks, 1L), steps), least = !p->chunk && most > 8 && steps > 16 ? 2 : 1;
+    kps = (int)std::max((steps + n - 1) / n, least) * PA_STEP;
   }
   p->tiles = (int)std::min<long>(tiles, 1 << 20);
   p->kps = kps;
@@ -395,7 +424,9 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
 
 template <int FMT, int D>
 void launch_attn(dim3 grid, hipStream_t st, const PaArgs& a) {
-  hipLaunchKernelGGL((paged_attn_kernel<FMT, D>), grid, dim3(256), 0, st, a);
+  constexpr bool FITS = FMT != QVEX_KV_BF16 || D == 128;         // 16 KB of K and of V per wave leave no registers over
+  if (FITS && a.kps > PA_STEP) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, FITS>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace

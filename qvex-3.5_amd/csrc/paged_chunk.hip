@@ -25,31 +25,6 @@ typedef float pc_f32x16 __attribute__((ext_vector_type(16)));
 constexpr int PC_KEYS = 64;            // keys per step
 constexpr int PC_AHEAD = 8;            // operands of the second-next products asked for ahead
 
-// Lane i of each 16-lane row, in every lane of that row.
-template <int I>
-__device__ __forceinline__ float row_lane(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + I, 0xf, 0xf, false));
-}
-__device__ __forceinline__ float row_lane_of(float v, int i) {   // i a constant after unrolling
-  switch (i) {
-    case 0: return row_lane<0>(v);
-    case 1: return row_lane<1>(v);
-    case 2: return row_lane<2>(v);
-    case 3: return row_lane<3>(v);
-    case 4: return row_lane<4>(v);
-    case 5: return row_lane<5>(v);
-    case 6: return row_lane<6>(v);
-    case 7: return row_lane<7>(v);
-    case 8: return row_lane<8>(v);
-    case 9: return row_lane<9>(v);
-    case 10: return row_lane<10>(v);
-    case 11: return row_lane<11>(v);
-    case 12: return row_lane<12>(v);
-    case 13: return row_lane<13>(v);
-    case 14: return row_lane<14>(v);
-    default: return row_lane<15>(v);
-  }
-}
 template <int I = 0>
 __device__ __forceinline__ void scale16(pc_f32x16& s, float v) {
   if constexpr (I < 16) {
@@ -425,7 +400,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         *reinterpret_cast<float4*>(a.ws + (((size_t)tok * a.Hq + head) * a.nsplit + split) * D + 4 * c) = v;
       } else {
         const float y[4] = {v.x, v.y, v.z, v.w};
-        pa_gate_store(a, tok, head, 4 * c, D, y);
+        PaGate(a, tok, head, 4 * c).store(a, tok, head, 4 * c, D, y);
       }
     }
     __syncthreads();

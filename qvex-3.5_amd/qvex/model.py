@@ -676,6 +676,7 @@ class Attention:
 
     # keys per split of the decode / verify attention (a multiple of 128)
     decode_kps = 128
+    paged_kps = 256         # the same over a paged cache (us, 4 rows at 7001 keys: 128 16, 256 15, 512 16)
     fused_decode = False    # qvex_attention_decode for 1..8 new tokens (slower per cycle: see its header)
     late_splits = True      # captured: splits past the position at capture read it before loading
 
@@ -708,7 +709,7 @@ class Attention:
         gate = proj[:, :2 * H * D].unflatten(1, (H, 2 * D))[..., D:]
         # one split length for the calls of a verify width: a row's bits are those of a plain step
         o = paged.attention(pages, q, cache.table, cache.pos, max_keys, gate=gate,
-                            keys_per_split=self.decode_kps if L <= 8 else 0)
+                            keys_per_split=self.paged_kps if L <= 8 else 0)
         return o.view(L, H * D)
 
     def __call__(self, x, cache: KVCache | paged.PagedKVCache, resid=None, norm_w=None, eps=None):
