@@ -68,6 +68,20 @@ __device__ __forceinline__ u32x4 codes8(uint32_t lo, uint32_t hi) {
   return o;
 }
 
+// Codes 2 t and 2 t + 1 of two keys' words x, y: as bf16 pairs (x, y).
+template <int FMT>
+__device__ __forceinline__ void pair2(uint32_t x, uint32_t y, int t, uint32_t& a0, uint32_t& a1) {
+  if constexpr (FMT == QVEX_KV_FP8) {
+    const uint32_t w = __builtin_amdgcn_perm(y, x, t & 1 ? 0x07030602u : 0x05010400u);
+    a0 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+    a1 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+  } else {
+    const int s = t & 1 ? 16 : 0;
+    a0 = pa_pack((float)(int8_t)(x >> s), (float)(int8_t)(y >> s));
+    a1 = pa_pack((float)(int8_t)(x >> (s + 8)), (float)(int8_t)(y >> (s + 8)));
+  }
+}
+
 // The A operands of tiles 2 t and 2 t + 1: values 2 t and 2 t + 1 of each of eight keys' runs v.
 template <int FMT, int VW>
 __device__ __forceinline__ void gather2(const uint32_t (&v)[8][VW], int t, u32x4& a0, u32x4& a1) {
@@ -77,16 +91,27 @@ __device__ __forceinline__ void gather2(const uint32_t (&v)[8][VW], int t, u32x4
       a0[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x05040100u);
       a1[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x07060302u);
     } else {
-      const uint32_t x = v[2 * i][t >> 1], y = v[2 * i + 1][t >> 1];
-      if constexpr (FMT == QVEX_KV_FP8) {
-        const uint32_t w = __builtin_amdgcn_perm(y, x, t & 1 ? 0x07030602u : 0x05010400u);
-        a0[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-        a1[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
-      } else {
-        const int s = t & 1 ? 16 : 0;
-        a0[i] = pa_pack((float)(int8_t)(x >> s), (float)(int8_t)(y >> s));
-        a1[i] = pa_pack((float)(int8_t)(x >> (s + 8)), (float)(int8_t)(y >> (s + 8)));
-      }
+      uint32_t x, y;
+      pair2<FMT>(v[2 * i][t >> 1], v[2 * i + 1][t >> 1], t, x, y);
+      a0[i] = x;
+      a1[i] = y;
+    }
+  }
+}
+
+// The same of four keys.
+template <int FMT, int VW>
+__device__ __forceinline__ void gather2x4(const uint32_t (&v)[4][VW], int t, u32x2& a0, u32x2& a1) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (FMT == QVEX_KV_BF16) {
+      a0[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x05040100u);
+      a1[i] = __builtin_amdgcn_perm(v[2 * i + 1][t], v[2 * i][t], 0x07060302u);
+    } else {
+      uint32_t x, y;
+      pair2<FMT>(v[2 * i][t >> 1], v[2 * i + 1][t >> 1], t, x, y);
+      a0[i] = x;
+      a1[i] = y;
     }
   }
 }

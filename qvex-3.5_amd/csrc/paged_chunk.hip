@@ -9,8 +9,8 @@
 //   of a 16-key step of the second product, whose A operand holds the same eight
 //   keys of one dim: V is stored in LDS by dims, its keys in that order.
 // LDS, in 16-byte units: K's row r holds unit c at c ^ (r % 16); V's row of dim d is
-// row d with its low two bits XORed by d / 16 % 4, unit c at c ^ (d / 4 % 4): the 16 lanes
-// of one pass of a read, and of a write, hit 16 different bank groups.
+// row d with its low two bits XORed by d / 16 % 4, unit c at c ^ (d / 4 % 4) ^ (d / 64): the 16
+// lanes of one pass of a read hit 16 different bank groups, and those of a write too.
 // A lane's 16 keys of a tile are one scale each for all its rows: a 16-lane row of
 // the wave holds them, and a product takes scale i by DPP broadcast.
 // Scores, m, l and O as in paged_attn.hip, but P is one bf16 term (2^-8 of a weight at
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
   constexpr int EB = kv_bytes(FMT), ROW = D * EB, KS = D / 16, NT = D / 32;
   constexpr int KU = PC_KEYS * ROW / 4096;       // 16-byte loads of K per thread and step
   constexpr int LPR = ROW / 16, KSTEP = 256 / LPR;   // lanes per key row, keys per load of the block
-  constexpr int VT = D / 128;                    // runs of (8 keys x 4 dims) of V per thread and step
+  constexpr int E = D / 16, VW = E * EB / 4;     // a thread's part of V and step: E dims (VW words) of four keys
   constexpr int K_BYTES = PC_KEYS * D * 2, STAGE = 2 * K_BYTES;
   __shared__ __align__(1024) uint8_t lds[2 * STAGE];
   __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
 
     // ---- a step's keys: pages to registers, registers to LDS
     u32x4 kraw[KU];
-    uint32_t vraw[VT][8][EB];
+    uint32_t vraw[4][VW];
     float ksn[2], vsn[2];
     uint32_t s0, s1, s2, s3;                                      // first slots of a step's 16-key groups
     int g0, g1, g2, g3;                                           // their pages, asked for a step before
@@ -119,20 +119,22 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         ksn[1] = scale_of(a.c.ks, 1);
       }
     };
+    const int vq = lane >> 4, vc = lane & 15;                     // keys 4 vq .. + 3 of the wave's 16, dims E vc .. + E - 1
     auto fetch_v = [&]() __attribute__((always_inline)) {
       const uint8_t* base = a.c.v + (uint64_t)pick(s0, s1, s2, s3, wave) * ROW;
 #pragma unroll
-      for (int t = 0; t < VT; ++t) {                              // the wave's 16 keys; half of them per run
-        const uint8_t* p = base + (uint32_t)(VT == 2 ? 4 * t * ROW + 4 * EB * lane : 4 * hf * ROW + 4 * EB * li);
+      for (int e = 0; e < 4; ++e) {
+        const uint8_t* p = base + (uint32_t)((4 * vq + e) * ROW + 4 * VW * vc);
+        if constexpr (VW == 2) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+          vraw[e][0] = w[0];
+          vraw[e][1] = w[1];
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint8_t* pe = p + (e + (e & 4)) * ROW;            // keys 0..3 and 8..11 of it
-          if constexpr (EB == 2) {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(pe);
-            vraw[t][e][0] = w[0];
-            vraw[t][e][1] = w[1];
-          } else {
-            vraw[t][e][0] = *reinterpret_cast<const uint32_t*>(pe);
+          for (int u = 0; u < VW / 4; ++u) {
+            const u32x4 w = load16(p + 16 * u);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) vraw[e][4 * u + x] = w[x];
           }
         }
       }
@@ -161,22 +163,20 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
       if constexpr (FMT != QVEX_KV_INT8) {
         const bool v_ok = ok_all >> wave & 1;
 #pragma unroll
-        for (int t = 0; t < VT; ++t)
+        for (int e = 0; e < 4; ++e) {
+          const int key = kb + 16 * wave + 4 * vq + e;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int key = kb + 16 * wave + 4 * (VT == 2 ? t : hf) + e + (e & 4);
-#pragma unroll
-            for (int u = 0; u < EB; ++u) {
-              const uint32_t w = key >= k_hi || !v_ok ? 0 : vraw[t][e][u], w1 = key > first_lim ? tame<FMT>(w) : w;
-              any |= w1 != w;
-              vraw[t][e][u] = w1;
-            }
+          for (int u = 0; u < VW; ++u) {
+            const uint32_t w = key >= k_hi || !v_ok ? 0 : vraw[e][u], w1 = key > first_lim ? tame<FMT>(w) : w;
+            any |= w1 != w;
+            vraw[e][u] = w1;
           }
+        }
       }
       if (any) odd = 1;
     };
     // Pieces of a step's way to LDS, K's and V's
-    constexpr int KP = EB == 2 ? KU : 2 * KU, VP = 2 * VT;
+    constexpr int KP = EB == 2 ? KU : 2 * KU, VP = E / 2;
     const int kw_at = ((KSTEP / 4) * wave + lane / LPR) * (2 * D);
     auto stage_k = [&](int to, int x) __attribute__((always_inline)) {
       const int u = EB == 2 ? x : x / 2, h = x & 1;
@@ -188,32 +188,38 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         *reinterpret_cast<u32x4*>(kr + (((2 * c + h) ^ key) << 4)) = codes8<FMT>(kraw[u][2 * h], kraw[u][2 * h + 1]);
       }
     };
+    // dims E vc + 2 x, + 1: four keys of each, a half of unit 2 (wave % 2) + vq % 2
+    const int vw_at = K_BYTES + (wave >> 1) * (D * 64) + 64 * E * vc + 8 * (vq >> 1);
     auto stage_v = [&](int to, int x) __attribute__((always_inline)) {
-      const int t = x / 2, u = x & 1, h = VT == 2 ? t : hf, d4 = VT == 2 ? lane : li, y = (d4 >> 2) & 3;
-      uint8_t* vr = lds + (to ^ (K_BYTES + (wave >> 1) * (D * 64) + 256 * d4 + (((2 * (wave & 1) + h) ^ (d4 & 3)) << 4)));
-      u32x4 b0, b1;                                               // dims 4 d4 + 2 u, + 1: their rows' low bits permuted
-      gather2<FMT, EB>(vraw[t], u, b0, b1);
-      *reinterpret_cast<u32x4*>(vr + ((2 * u) ^ y) * 64) = b0;
-      *reinterpret_cast<u32x4*>(vr + ((2 * u + 1) ^ y) * 64) = b1;
+      u32x2 b0, b1;
+      gather2x4<FMT, VW>(vraw, x, b0, b1);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int n = 2 * x + y;
+        const int r = (n & 3) ^ (E == 16 ? vc & 3 : (vc >> 1) & 3);
+        const int f = E == 16 ? ((n >> 2) ^ (vc >> 2)) & 3 : ((2 * vc + (n >> 2)) ^ (vc >> 3)) & 3;
+        *reinterpret_cast<u32x2*>(lds + (to ^ vw_at) + (n & ~3) * 64 + r * 64 + (((2 * (wave & 1) + (vq & 1)) ^ f) << 4)) =
+            y ? b1 : b0;
+      }
     };
 
     // ---- operands from LDS: K's of both key tiles, then V's. The lane's addresses are kept, the buffer's bit flipped
-    int k_at[KS < 8 ? KS : 8], v_at[2][2];                        // K: step st at entry st % 8, + 256 from 8
+    int k_at[KS < 8 ? KS : 8], v_at[2][4];                        // K: step st at entry st % 8, + 256 from 8
 #pragma unroll
     for (int st = 0; st < KS && st < 8; ++st) k_at[st] = li * (2 * D) + (((2 * st + hf) ^ (li & 15)) << 4);
 #pragma unroll
-    for (int x = 0; x < 2; ++x)                                   // V: even and odd dim tiles, 16-key steps
+    for (int x = 0; x < 2; ++x)                                   // V: even and odd dim tiles; 2 t ^ (n / 2)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        v_at[x][t] = K_BYTES + ((32 * x + (li & ~3)) | ((li & 3) ^ ((2 * x + (li >> 4)) & 3))) * 64 +
-                     (((2 * t + hf) ^ ((li >> 2) & 3)) << 4);
+      for (int y = 0; y < 4; ++y)
+        v_at[x][y] = K_BYTES + ((32 * x + (li & ~3)) | ((li & 3) ^ ((2 * x + (li >> 4)) & 3))) * 64 +
+                     ((hf ^ y ^ ((li >> 2) & 3)) << 4);
     auto operand = [&](int x) __attribute__((always_inline)) {
       if (x < 2 * KS) {
         const int kt = x / KS, st = x % KS;
         return load16(lds + k_at[st % 8] + (kt * 64 * D + (st >> 3) * 256));
       }
       const int y = x - 2 * KS, kt = y / (2 * NT), t = y / NT % 2, n = y % NT;
-      return load16(lds + v_at[n & 1][t] + (kt * (D * 64) + (n >> 1) * 4096));
+      return load16(lds + v_at[n & 1][(2 * t) ^ ((n >> 1) & 3)] + (kt * (D * 64) + (n >> 1) * 4096));
     };
 
     const pc_f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
 #pragma unroll
       for (int x = 0; x < KS && x < 8; ++x) k_at[x] ^= STAGE;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v_at[x >> 1][x & 1] ^= STAGE;
+      for (int x = 0; x < 8; ++x) v_at[x >> 2][x & 3] ^= STAGE;
       ok = ok_next;
       ok_next = ok_further;
       __syncthreads();
