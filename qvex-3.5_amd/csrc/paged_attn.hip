@@ -425,7 +425,9 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
 template <int FMT, int D>
 void launch_attn(dim3 grid, hipStream_t st, const PaArgs& a) {
   constexpr bool FITS = FMT != QVEX_KV_BF16 || D == 128;         // 16 KB of K and of V per wave leave no registers over
-  if (FITS && a.kps > PA_STEP) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, FITS>), grid, dim3(256), 0, st, a);
+  // many rows: other tiles' waves hide the loads, and fewer registers are worth more (us, two rows' tiles or more, with |
+  // without: 12 x 200 rows at 1500 keys 27.9 | 26.8; 2 x 64 at 1000 25.0 | 23.6; 16 x 12 at 2000 39.4 | 38.3)
+  if (FITS && a.kps > PA_STEP && a.r.L <= 8) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, FITS>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false>), grid, dim3(256), 0, st, a);
 }
 
