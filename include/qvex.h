@@ -591,7 +591,8 @@ int qvex_rope_table(int rot_dim, float theta, int rows, float* table, void* stre
  * KVCache (engine/model.py:149-176) keeps one dense array per sequence instead.
  *
  * A pool holds n_pages pages of `page` positions (a power of two, 16..1024) of
- * every kv head, K and V each [n_pages][Hkv][page][D] row-major, D 128 or 256:
+ * every kv head, K and V each [n_pages][Hkv][page][D] row-major, D 128 or 256,
+ * n_pages * Hkv * page below 2^31:
  *   QVEX_KV_BF16: bf16 values;
  *   QVEX_KV_INT8: codes c in -127..127, value = scale * c;
  *   QVEX_KV_FP8:  e4m3 codes (OCP, largest 448), value = scale * c;
@@ -653,10 +654,11 @@ int qvex_paged_read(const qvex_kv_pages* pages, const qvex_kv_rows* rows, void* 
                     int out_f32, void* stream);
 
 /* Causal GQA attention of the rows over their sequences' pages: row i of sequence
- * b sees positions 0 .. pos[b] + i, scores scaled by `scale` (>= 0), out [T, Hq, D] bf16 (a row
- * that sees nothing gets zeros; an infinity or a NaN among the values leaves that dim of
- * the rows that see it not finite, and no other row's). q: row t, head h at q + t*q_token + h*q_head; gate
- * (or NULL): alike, out times sigmoid(gate). max_keys bounds pos[b] + rows of every
+ * b sees positions 0 .. pos[b] + i, scores scaled by `scale` (>= 0), out
+ * [T, Hq, D] bf16 (a row that sees nothing gets zeros; an infinity or a NaN among the
+ * values leaves that dim of the rows that see it not finite, and no other row's). q:
+ * row t, head h at q + t*q_token + h*q_head; gate (or NULL): alike, out times
+ * sigmoid(gate). max_keys bounds pos[b] + rows of every
  * sequence (a larger one is still right, only slower). keys_per_split: keys per
  * block of a row's split (a multiple of 128), or 0 to choose by the call's size;
  * at one positive value a row's bits do not depend on the other rows of the call,

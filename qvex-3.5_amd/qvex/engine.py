@@ -73,8 +73,8 @@ def generate(model: Qwen35, prompt_ids, params: SamplingParams, mtp: MTPHead | N
     (engine/engine.py:280-300). `forced` is shared with the
     generator: ids appended to it while iterating are emitted next, as the
     reference's reasoning budget does. A stop id counts in completion_tokens but
-    is not returned. kv: how keys and values are kept (Qwen35.make_cache). Stats keys follow the reference's (engine/engine.py:340-357)
-    where they apply to this path."""
+    is not returned. kv: how keys and values are kept (Qwen35.make_cache). Stats keys
+    follow the reference's (engine/engine.py:340-357) where they apply to this path."""
     use_mtp = mtp_policy(mtp_mode, mtp)
     ids = torch.as_tensor(prompt_ids, dtype=torch.int32).reshape(1, -1).to(model.norm.device)
     if ids.shape[1] < 1:

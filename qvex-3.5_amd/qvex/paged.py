@@ -271,9 +271,11 @@ def _workspace_bytes(*args) -> int:
 
 def workspace_bytes(pages: KVPages, B: int, T: int, Hq: int, max_keys: int, max_rows: int | None = None,
                     keys_per_split: int = 0) -> int:
-    """Bytes of workspace that attention() takes for T rows of B sequences (0: none)."""
-    L = (T // B if T % B == 0 else T) if max_rows is None else max(1, min(int(max_rows), T))
-    return _workspace_bytes(B, L, T, Hq, pages.n_kv, pages.head_dim, int(max_keys), int(keys_per_split))
+    """Bytes of workspace that attention() takes for T rows of B sequences (0: none), with cu or
+    without. max_keys as there, at most the table's capacity."""
+    widths = {T, T // B} if max_rows is None else {max(1, min(int(max_rows), T))}
+    return max(_workspace_bytes(B, L, T, Hq, pages.n_kv, pages.head_dim, int(max_keys), int(keys_per_split))
+               for L in widths)
 
 
 # ---------------------------------------------------------------- pages handed to sequences
@@ -399,9 +401,9 @@ class PagedKVCache:
         self.table[0, :len(self.ids)].copy_(torch.tensor(self.ids, dtype=torch.int32))
 
     def _own(self, at: int) -> None:
-        """The pages from position `at` on become this cache's alone."""
+        """The pages from position `at` on become this cache's alone (those behind `offset` are)."""
         first, changed = at // self.pool.page, False
-        for x in range(first, len(self.ids)):
+        for x in range(first, min(self.offset // self.pool.page + 1, len(self.ids))):
             j = self.ids[x]
             if self.pool.holders[j] > 1:
                 self.ids[x] = self.pool.take(1)[0]

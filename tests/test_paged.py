@@ -219,6 +219,16 @@ def test_pool_grows_and_keeps_its_pages(fmt):
         assert torch.equal(a[:2], b)
 
 
+def test_workspace_of_a_call_with_and_without_row_offsets():
+    """max_rows left out: enough for T / B rows each and for all of them in one sequence."""
+    pages = paged.KVPages.alloc(64, 4, 256, "int8", 64, "cpu")
+    f = _C.lib().qvex_paged_attention_workspace_bytes
+    for B, T, mk in ((1, 1, 4000), (8, 64, 4000), (64, 64, 2000), (3, 100, 4000), (4, 512, 4096)):
+        got = paged.workspace_bytes(pages, B, T, 16, mk)
+        assert got == max(f(B, L, T, 16, 4, 256, mk, 0) for L in (max(T // B, 1), T))
+    assert paged.workspace_bytes(pages, 4, 0, 16, 100) == 0
+
+
 def test_cache_grows_without_moving_and_returns_its_pages():
     pool = paged.PagePool(40, 2, 128, "fp8", 16, "cpu")
     c = paged.PagedKVCache(pool, capacity=100)
