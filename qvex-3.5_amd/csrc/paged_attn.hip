@@ -33,7 +33,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
   __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int li = lane & 15, lg = lane >> 4;
-  const int b = blockIdx.y, split = blockIdx.z, kh = blockIdx.x % a.c.Hkv, GQ = a.Hq / a.c.Hkv;
+  const KvBlock blk(a.r, a.c.Hkv);
+  const int b = blk.pair / a.c.Hkv, kh = blk.pair - b * a.c.Hkv, split = blockIdx.z, GQ = a.Hq / a.c.Hkv;
   const KvSeq s(a.r, b);
   const int cap = a.r.width << a.c.shift, rows = s.n * GQ, mask = (1 << a.c.shift) - 1;
   const int32_t* table = a.r.table + b * a.r.stride;
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
   };
   const int first0 = page_at(k_lo + 32 * wave), first1 = page_at(k_lo + 32 * wave + 16);
 
-  for (int tile = blockIdx.x / a.c.Hkv; tile * PA_ROWS < rows; tile += gridDim.x / a.c.Hkv) {
+  for (int tile = blk.piece; tile * PA_ROWS < rows; tile += gridDim.y) {
     const int row = tile * PA_ROWS + li, last = min(rows, (tile + 1) * PA_ROWS) - 1;
     const bool used = row < rows;
     const int i = used ? row / GQ : 0, g = used ? row - i * GQ : 0;
@@ -295,13 +296,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 
   // rows of sequences without a visible key (a negative position): nobody else writes them
   if (a.nsplit == 1 && s.pos < 0) {
-    for (int w = blockIdx.x / a.c.Hkv; w < s.n && s.pos + w < 0; w += gridDim.x / a.c.Hkv)
+    for (int w = blk.piece; w < s.n && s.pos + w < 0; w += gridDim.y)
       for (int x = threadIdx.x; x < GQ * D; x += 256) a.out[((size_t)(s.first + w) * a.Hq + kh * GQ) * D + x] = 0;
   }
 }
 
 // A call of more than 8 rows per sequence takes the chunk form (paged_chunk.hip) if a sequence's
-// rows of a kv head fill half a block and (query, key) pairs * D are worth its start and end,
+// rows of a kv head fill half a block (a quarter on average, whatever L allows) and (query, key) pairs * D are worth its start and end,
 // 8 us against 3. us, this form | that one, int8, 16 query and 4 kv heads of 256 (pairs = T * Hq *
 // max_keys): 64 positions at 1000 keys (1.1M) 23 | 24, at 4000 (4.2M) 34 | 33, 512 at 0 (4.2M) 30 | 27,
 // 8 x 64 at 1000 (8.7M) 47 | 39, at 4000 (33M) 111 | 72, 512 at 4000 (37M) 119 | 75; of 128, 4 and 2
@@ -319,12 +320,13 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
   constexpr int LANES = D / 4, PER = 256 / LANES, BATCH = 8, STEP = WIDE ? PER : 1;
   __shared__ __align__(16) float part[WIDE ? PER : 1][D];
   __shared__ float2 pml[WIDE ? PER : 1];
-  const int b = blockIdx.y, sub = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+  const KvBlock blk(a.r, 1);
+  const int b = blk.pair, sub = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
   const KvSeq s(a.r, b);
   const int cap = a.r.width << a.c.shift;
   const long rows = (long)s.n * a.Hq;
   const int each = WIDE ? 1 : PER;
-  for (long w = (long)blockIdx.x * each + (WIDE ? 0 : sub); w < rows; w += (long)gridDim.x * each) {
+  for (long w = (long)blk.piece * each + (WIDE ? 0 : sub); w < rows; w += (long)gridDim.y * each) {
     const int i = (int)(w / a.Hq), h = (int)(w - (long)i * a.Hq), tok = s.first + i;
     const size_t rec = ((size_t)tok * a.Hq + h) * a.nsplit;
     const float2* mls = pa_ml(a, D) + rec;
@@ -402,20 +404,24 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
       max_keys > KV_LIMIT || kps < 0 || kps % PA_STEP)
     return false;
   const long GQ = Hq / Hkv, most = std::min(L, std::max(T, 1)) * GQ;
-  p->chunk = L > 8 && most >= PA_CHUNK_MIN && (double)T * Hq * max_keys * D >= PA_CHUNK_WORK;
+  p->chunk = L > 8 && most >= PA_CHUNK_MIN && (double)T * GQ >= 0.5 * PA_CHUNK_MIN * B &&
+             (double)T * Hq * max_keys * D >= PA_CHUNK_WORK;
   const int per = p->chunk ? qvex::PA_CHUNK_ROWS : PA_ROWS;
-  const long tiles = (most + per - 1) / per, steps = (max_keys + PA_STEP - 1) / PA_STEP;
+  const long full = (long)T * GQ / per + B, steps = (max_keys + PA_STEP - 1) / PA_STEP;   // tiles with rows, at most
+  // where L says little of a sequence (every row of the call may be one's), few of B * tiles have rows: the blocks
+  // of the longest sequence then take several
+  const long tiles = std::min((most + per - 1) / per, std::max(4 * full, 4096L) / B + 1);
   if (kps == 0) {
     // as many splits as give each CU a block (us, int8, 256-dim heads, blocks of one split | n splits: 16
     // x 2000 keys (64 blocks) 28 | 4: 18 | 16: 22; 8 x 4 rows at 4096 (32) 54 | 8: 21 | 33: 30; 64 x 4600 (256) 112
     // | 2: 112 | 36: 154), of two steps at least where a tile is more than half full (its
     // records cost more than the second step: 4 rows at 7001 keys 16 | 14)
-    const long blocks = std::max(std::min(B * tiles, T * GQ / per + B) * Hkv, 1L);
+    const long blocks = std::max(std::min(B * tiles, full) * Hkv, 1L);
     const long want = p->chunk || L <= 8 ? 256 : 768;             // many row tiles of unequal lengths
     const long n = std::min(std::max(want / blocks, 1L), steps), least = !p->chunk && most > 8 && steps > 16 ? 2 : 1;
     kps = (int)std::max((steps + n - 1) / n, least) * PA_STEP;
   }
-  p->tiles = (int)std::min<long>(tiles, 1 << 20);
+  p->tiles = (int)std::min(tiles, 65535L);
   p->kps = kps;
   p->nsplit = (max_keys - 1) / kps + 1;
   p->bytes = p->nsplit == 1 ? 0 : (uint64_t)T * Hq * p->nsplit * (D + 2) * sizeof(float);
@@ -451,7 +457,7 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
   QVEX_CHECK_ARG(pa_plan(B, a.r.L, a.r.T, Hq, a.c.Hkv, D, max_keys, keys_per_split, &p) && Hq <= 16384,
                  "%s: Hq=%d Hkv=%d max_keys=%d keys_per_split=%d (a multiple of 128, or 0)", fn, Hq, a.c.Hkv, max_keys,
                  keys_per_split);
-  QVEX_CHECK_ARG(p.nsplit <= 65535, "%s: grid too large", fn);
+  QVEX_CHECK_ARG(p.nsplit <= 65535 && (long)B * a.c.Hkv < 1 << 24, "%s: grid too large", fn);
   QVEX_CHECK_ARG(scale >= 0.0f && scale < INFINITY, "%s: scale=%g must be finite, not negative", fn, (double)scale);
   if (a.r.T == 0) return QVEX_OK;
   QVEX_CHECK_ARG(q && out && qvex_aligned(q, 2) && qvex_aligned(out, 16) && qvex_aligned(gate, 2),
@@ -473,7 +479,7 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
   a.vec = (q_token % 8 | q_head % 8) == 0 && qvex_aligned(q, 16);
   a.c2 = fmaxf(scale * 1.44269504088896340736f, 1e-37f);       // a masked score stays -inf at a scale of 0 too
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(a.c.Hkv * p.tiles, B, p.nsplit);
+  const dim3 grid(a.c.Hkv * B, p.tiles, p.nsplit);
   const int f = pages->format;
   const auto go = D == 256 ? (f == QVEX_KV_BF16   ? &launch_attn<QVEX_KV_BF16, 256>
                               : f == QVEX_KV_INT8 ? &launch_attn<QVEX_KV_INT8, 256>
@@ -489,7 +495,7 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
     const bool wide = a.r.L <= 8;
     const int per = wide ? 1 : 256 / (D / 4);
     const long most = (8192 + B - 1) / B, want = ((long)a.r.L * Hq + per - 1) / per;
-    const dim3 mgrid((unsigned)std::min(want, most), B);
+    const dim3 mgrid(B, (unsigned)std::min(want, most));
     const auto merge = D == 256 ? (wide ? &paged_attn_merge_kernel<256, true> : &paged_attn_merge_kernel<256, false>)
                                 : (wide ? &paged_attn_merge_kernel<128, true> : &paged_attn_merge_kernel<128, false>);
     hipLaunchKernelGGL(merge, mgrid, dim3(256), 0, st, a);

@@ -279,6 +279,43 @@ def test_attention_of_prompt_chunks(dev, fmt, kps, D, Hq, n_kv, page, lens, pos)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,Hq,n_kv,page,lens,wide", [
+    (128, 4, 1, 16, [500] + [1, 0, 2] * 40, False),     # more tiles than the longest sequence gets blocks
+    (128, 4, 2, 32, [70] + [1] * 63, False), (256, 4, 1, 16, [1] * 33 + [40] + [2] * 30, False),
+    (128, 4, 1, 16, [600] + [3, 0, 9] * 13, True), (256, 8, 2, 64, [5, 0, 130, 1], True),
+])
+@pytest.mark.parametrize("bound", [False, True])
+def test_attention_of_unequal_sequences(dev, fmt, D, Hq, n_kv, page, lens, wide, bound):
+    pos = [(37 * b) % 90 for b in range(len(lens))]
+    check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, wide=wide, max_rows=max(lens) if bound else None)
+
+
+def test_append_read_and_input_stage_of_unequal_sequences(dev):
+    """Every row of a batch of one long and many short sequences, as in a call of its own."""
+    D, Hq, n_kv, page, lens = 128, 4, 2, 16, [300] + [1, 0, 3] * 30 + [64]
+    pos = [(5 * b) % 50 for b in range(len(lens))]
+    T, cu = sum(lens), i32(offsets(lens), dev)
+    table, n_pages = layout(lens, pos, page, 31)
+    table, posd = i32(table.tolist(), dev), i32(pos, dev)
+    proj = torch.randn((T, Hq * 2 * D + 2 * n_kv * D), generator=gen(32)).to(BF16).to(dev)
+    w, freqs = torch.ones(D, dtype=BF16, device=dev), paged.rope_freqs(64, 1e6, dev)
+    a, b, c = (paged.KVPages.alloc(n_pages, n_kv, D, "int8", page, dev) for _ in range(3))
+    q = paged.attn_qk_rope(a, proj, w, w, table, posd, freqs, 1e-6, cu)
+    kv = torch.randn((T, n_kv, D), generator=gen(33)).to(BF16).to(dev)
+    paged.kv_append(c, kv, kv, table, posd, cu)
+    k, _ = paged.kv_read(c, table, posd, T, cu)
+    for s, n in enumerate(lens):
+        if n:
+            at = slice(sum(lens[:s]), sum(lens[:s + 1]))
+            one = (table[s:s + 1].contiguous(), posd[s:s + 1])
+            assert torch.equal(q[at], paged.attn_qk_rope(b, proj[at], w, w, *one, freqs, 1e-6))
+            assert torch.equal(k[at], paged.kv_read(c, *one, n)[0])
+    for x, y in zip(a.tensors(), b.tensors()):
+        assert torch.equal(x, y)
+    assert float((k.float() - kv.float()).abs().max()) <= float(kv.float().abs().max()) * (0.5 / 127 + 2.0 ** -8)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("kps,max_keys", [(128, None), (256, 1200), (0, 1), (128, 130), (1152, None)])
 def test_attention_splits(dev, fmt, kps, max_keys):
     """Any split, and a bound on the keys that is too small."""
