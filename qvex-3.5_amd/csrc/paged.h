@@ -49,32 +49,6 @@ __device__ __forceinline__ long kv_slot(const KvPages& c, const KvRows& r, int b
   return (((long)page * c.Hkv + head) << c.shift) + (p & ((1 << c.shift) - 1));
 }
 
-// A block's work: piece `piece` of sequence `pair` (times `heads`, plus a head); the grid is [B * heads][pieces].
-// Workgroups go round the 8 XCDs and their engines in order of their number. Sequences of one
-// length: a sequence's pieces are neighbours, and read its keys at one time (us, 64 x 8 rows after 2000 bf16
-// keys: 152; rotated 170). Row offsets: sequences may leave blocks without work, so blocks with
-// work must not lie a power of two apart: first pieces are neighbours, and each further row of the
-// grid is rotated, so that the pieces of one sequence are too (us, int8 after 2000 to 4000 keys, 64
-// sequences of one row, bound 64 | one of 512 rows and 63 of one | one of 512 and 15 of one, pieces as
-// neighbours 420 | 773 | 166, not rotated 102 | 327 | 527, rotated 103 | 221 | 193).
-struct KvBlock {
-  int pair, piece;
-  __device__ __forceinline__ KvBlock(const KvRows& r, int heads) {
-    const uint32_t x = blockIdx.x, y = blockIdx.y, n = gridDim.x, pieces = gridDim.y;
-    pair = x;
-    piece = y;
-    if (pieces == 1) return;
-    if (r.cu) {
-      const uint32_t turn = y * ((64 + heads - n) & 63) % n;
-      pair = x < turn ? x + n - turn : x - turn;
-    } else {
-      const uint32_t at = y * n + x, row = at / heads, s = row / pieces;
-      piece = row - s * pieces;
-      pair = s * heads + (at - row * heads);
-    }
-  }
-};
-
 constexpr int kv_bytes(int format) { return format == QVEX_KV_BF16 ? 2 : 1; }
 
 // Checks the two structs; on success *pc and *rc are what the kernels take.

@@ -42,6 +42,39 @@ __device__ __forceinline__ int pa_page(const int32_t* t, int i) {
   return ((const __attribute__((address_space(4))) int32_t*)t)[i];
 }
 
+// A block's work: row tiles `tile`, `tile` + `tiles`, ... of kv head kh of sequence b. Workgroups go round
+// the 8 XCDs and their engines in order of their number. Sequences of one length, grid
+// [tiles * Hkv][B]: a sequence's tiles are neighbours, and read its keys at one time (us, 64 x 8 rows after 2000 bf16
+// keys: 152; as below 170). With row offsets, sequences may leave blocks without rows, so blocks with
+// rows must not lie a power of two apart: grid [B * Hkv][tiles], first tiles are neighbours, and each
+// further row of the grid is rotated, so that the tiles of one sequence are too (us, int8 after 2000
+// to 4000 keys, 64 sequences of one row, bound 64 | one of 512 rows and 63 of one | one of 512 and 15 of
+// one, a sequence's tiles as neighbours 420 | 773 | 166, not rotated 102 | 327 | 527, rotated 106 | 223 | 189).
+struct PaBlock {
+  int b, kh, tile, tiles;
+  __device__ __forceinline__ PaBlock(const PaArgs& a) {
+    const uint32_t x = blockIdx.x, y = blockIdx.y, n = gridDim.x, heads = a.c.Hkv;
+    uint32_t pair = x;
+    if (a.r.cu) {
+      const uint32_t turn = y == 0 ? 0 : y * ((64 + heads - n) & 63) % n;
+      pair = x < turn ? x + n - turn : x - turn;
+      b = pair / heads;
+      tile = y;
+      tiles = gridDim.y;
+    } else {
+      b = y;
+      tile = x / heads;
+      tiles = n / heads;
+      pair = x - tile * heads;
+    }
+    kh = a.r.cu ? pair - b * heads : pair;
+  }
+};
+
+inline dim3 pa_grid(const PaArgs& a, int B, int tiles) {
+  return a.r.cu ? dim3(a.c.Hkv * B, tiles, a.nsplit) : dim3(a.c.Hkv * tiles, B, a.nsplit);
+}
+
 __device__ __forceinline__ u32x4 pa_load8(const uint16_t* p, int vec) {
   if (vec) return load16(p);
   u32x4 w;

@@ -33,8 +33,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
   __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int li = lane & 15, lg = lane >> 4;
-  const KvBlock blk(a.r, a.c.Hkv);
-  const int b = blk.pair / a.c.Hkv, kh = blk.pair - b * a.c.Hkv, split = blockIdx.z, GQ = a.Hq / a.c.Hkv;
+  const PaBlock blk(a);
+  const int b = blk.b, kh = blk.kh, split = blockIdx.z, GQ = a.Hq / a.c.Hkv;
   const KvSeq s(a.r, b);
   const int cap = a.r.width << a.c.shift, rows = s.n * GQ, mask = (1 << a.c.shift) - 1;
   const int32_t* table = a.r.table + b * a.r.stride;
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
   };
   const int first0 = page_at(k_lo + 32 * wave), first1 = page_at(k_lo + 32 * wave + 16);
 
-  for (int tile = blk.piece; tile * PA_ROWS < rows; tile += gridDim.y) {
+  for (int tile = blk.tile; tile * PA_ROWS < rows; tile += blk.tiles) {
     const int row = tile * PA_ROWS + li, last = min(rows, (tile + 1) * PA_ROWS) - 1;
     const bool used = row < rows;
     const int i = used ? row / GQ : 0, g = used ? row - i * GQ : 0;
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 
   // rows of sequences without a visible key (a negative position): nobody else writes them
   if (a.nsplit == 1 && s.pos < 0) {
-    for (int w = blk.piece; w < s.n && s.pos + w < 0; w += gridDim.y)
+    for (int w = blk.tile; w < s.n && s.pos + w < 0; w += blk.tiles)
       for (int x = threadIdx.x; x < GQ * D; x += 256) a.out[((size_t)(s.first + w) * a.Hq + kh * GQ) * D + x] = 0;
   }
 }
@@ -320,13 +320,12 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
   constexpr int LANES = D / 4, PER = 256 / LANES, BATCH = 8, STEP = WIDE ? PER : 1;
   __shared__ __align__(16) float part[WIDE ? PER : 1][D];
   __shared__ float2 pml[WIDE ? PER : 1];
-  const KvBlock blk(a.r, 1);
-  const int b = blk.pair, sub = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+  const int b = blockIdx.y, sub = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
   const KvSeq s(a.r, b);
   const int cap = a.r.width << a.c.shift;
   const long rows = (long)s.n * a.Hq;
   const int each = WIDE ? 1 : PER;
-  for (long w = (long)blk.piece * each + (WIDE ? 0 : sub); w < rows; w += (long)gridDim.y * each) {
+  for (long w = (long)blockIdx.x * each + (WIDE ? 0 : sub); w < rows; w += (long)gridDim.x * each) {
     const int i = (int)(w / a.Hq), h = (int)(w - (long)i * a.Hq), tok = s.first + i;
     const size_t rec = ((size_t)tok * a.Hq + h) * a.nsplit;
     const float2* mls = pa_ml(a, D) + rec;
@@ -421,7 +420,7 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
     const long n = std::min(std::max(want / blocks, 1L), steps), least = !p->chunk && most > 8 && steps > 16 ? 2 : 1;
     kps = (int)std::max((steps + n - 1) / n, least) * PA_STEP;
   }
-  p->tiles = (int)std::min(tiles, 65535L);
+  p->tiles = (int)std::min(tiles, 65535L);   // of a grid
   p->kps = kps;
   p->nsplit = (max_keys - 1) / kps + 1;
   p->bytes = p->nsplit == 1 ? 0 : (uint64_t)T * Hq * p->nsplit * (D + 2) * sizeof(float);
@@ -479,7 +478,7 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
   a.vec = (q_token % 8 | q_head % 8) == 0 && qvex_aligned(q, 16);
   a.c2 = fmaxf(scale * 1.44269504088896340736f, 1e-37f);       // a masked score stays -inf at a scale of 0 too
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(a.c.Hkv * B, p.tiles, p.nsplit);
+  const dim3 grid = pa_grid(a, B, p.tiles);
   const int f = pages->format;
   const auto go = D == 256 ? (f == QVEX_KV_BF16   ? &launch_attn<QVEX_KV_BF16, 256>
                               : f == QVEX_KV_INT8 ? &launch_attn<QVEX_KV_INT8, 256>
@@ -495,7 +494,7 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
     const bool wide = a.r.L <= 8;
     const int per = wide ? 1 : 256 / (D / 4);
     const long most = (8192 + B - 1) / B, want = ((long)a.r.L * Hq + per - 1) / per;
-    const dim3 mgrid(B, (unsigned)std::min(want, most));
+    const dim3 mgrid((unsigned)std::min(want, most), B);
     const auto merge = D == 256 ? (wide ? &paged_attn_merge_kernel<256, true> : &paged_attn_merge_kernel<256, false>)
                                 : (wide ? &paged_attn_merge_kernel<128, true> : &paged_attn_merge_kernel<128, false>);
     hipLaunchKernelGGL(merge, mgrid, dim3(256), 0, st, a);

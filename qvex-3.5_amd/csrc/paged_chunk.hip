@@ -51,14 +51,14 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
   __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int li = lane & 31, hf = lane >> 5;
-  const KvBlock blk(a.r, a.c.Hkv);
-  const int b = blk.pair / a.c.Hkv, kh = blk.pair - b * a.c.Hkv, split = blockIdx.z, GQ = a.Hq / a.c.Hkv;
+  const PaBlock blk(a);
+  const int b = blk.b, kh = blk.kh, split = blockIdx.z, GQ = a.Hq / a.c.Hkv;
   const KvSeq s(a.r, b);
   const int cap = a.r.width << a.c.shift, rows = s.n * GQ, mask = (1 << a.c.shift) - 1;
   const int32_t* table = a.r.table + b * a.r.stride;
   const int k_lo = split * a.kps;
 
-  for (int tile = blk.piece; tile * qvex::PA_CHUNK_ROWS < rows; tile += gridDim.y) {
+  for (int tile = blk.tile; tile * qvex::PA_CHUNK_ROWS < rows; tile += blk.tiles) {
     const int r0 = tile * qvex::PA_CHUNK_ROWS;
     const int last = min(rows, r0 + qvex::PA_CHUNK_ROWS) - 1;
     const int keys = min(s.pos + last / GQ + 1, cap);             // that any row of the block sees
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
 
   // rows without a visible key in a call of one split: nobody else writes them
   if (a.nsplit == 1 && s.pos < 0) {
-    for (int w = blk.piece; w < s.n && s.pos + w < 0; w += gridDim.y)
+    for (int w = blk.tile; w < s.n && s.pos + w < 0; w += blk.tiles)
       for (int x = threadIdx.x; x < GQ * D; x += 256) a.out[((size_t)(s.first + w) * a.Hq + kh * GQ) * D + x] = 0;
   }
 }
@@ -430,7 +430,7 @@ void launch(int D, dim3 grid, hipStream_t st, const PaArgs& a) {
 
 void qvex::paged_chunk_attention(const void* args, int format, int D, int tiles, int B, void* stream) {
   const PaArgs& a = *static_cast<const PaArgs*>(args);
-  const dim3 grid(a.c.Hkv * B, tiles, a.nsplit);
+  const dim3 grid = pa_grid(a, B, tiles);
   const auto go = format == QVEX_KV_BF16 ? &launch<QVEX_KV_BF16> : format == QVEX_KV_INT8 ? &launch<QVEX_KV_INT8> : &launch<QVEX_KV_FP8>;
   go(D, grid, (hipStream_t)stream, a);
 }

@@ -83,11 +83,10 @@ __global__ __launch_bounds__(KV_THREADS) void paged_append_kernel(KvPages c, KvR
                                                                   const uint16_t* __restrict__ v, long v_token,
                                                                   long v_head, int vec) {
   constexpr int PER = KV_THREADS / LANES;
-  const KvBlock blk(r, 1);
-  const int b = blk.pair, lane = threadIdx.x % LANES;
+  const int b = blockIdx.y, lane = threadIdx.x % LANES;
   const KvSeq s(r, b);
   const long rows = (long)s.n * c.Hkv * 2;
-  for (long w = (long)blk.piece * PER + threadIdx.x / LANES; w < rows; w += (long)gridDim.y * PER) {
+  for (long w = (long)blockIdx.x * PER + threadIdx.x / LANES; w < rows; w += (long)gridDim.x * PER) {
     const bool isv = w & 1;
     const int h = (int)((w >> 1) % c.Hkv), i = (int)((w >> 1) / c.Hkv);
     const uint16_t* src = isv ? v + (s.first + i) * v_token + h * v_head : k + (s.first + i) * k_token + h * k_head;
@@ -109,12 +108,11 @@ __global__ __launch_bounds__(KV_THREADS) void paged_qk_rope_kernel(KvPages c, Kv
   constexpr int D = 8 * LANES, PER = KV_THREADS / LANES;
   __shared__ float2 turn[D / 2];
   __shared__ float rowbuf[PER][D];
-  const KvBlock blk(r, 1);
-  const int b = blk.pair, lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, half = rot / 2;
+  const int b = blockIdx.y, lane = threadIdx.x % LANES, sub = threadIdx.x / LANES, half = rot / 2;
   const KvSeq s(r, b);
   const int heads = Hq + 2 * c.Hkv, groups = (heads + PER - 1) / PER;
   const double freq = (int)threadIdx.x < half ? freqs[threadIdx.x] : 0.0;
-  for (long w = blk.piece; w < (long)s.n * groups; w += gridDim.y) {     // uniform over the block
+  for (long w = blockIdx.x; w < (long)s.n * groups; w += gridDim.x) {     // uniform over the block
     const int i = (int)(w / groups), h = (int)(w % groups) * PER + sub, p = s.pos + i;
     const bool used = h < heads, isq = h < Hq, isv = h >= Hq + c.Hkv;
     const int kh = isv ? h - Hq - c.Hkv : h - Hq;
@@ -193,11 +191,10 @@ template <int FMT, int LANES, typename OUT>
 __global__ __launch_bounds__(KV_THREADS) void paged_read_kernel(KvPages c, KvRows r, OUT* __restrict__ k_out,
                                                                 OUT* __restrict__ v_out) {
   constexpr int D = 8 * LANES, PER = KV_THREADS / LANES, ROW = D * kv_bytes(FMT);
-  const KvBlock blk(r, 1);
-  const int b = blk.pair, lane = threadIdx.x % LANES;
+  const int b = blockIdx.y, lane = threadIdx.x % LANES;
   const KvSeq s(r, b);
   const long rows = (long)s.n * c.Hkv * 2;
-  for (long w = (long)blk.piece * PER + threadIdx.x / LANES; w < rows; w += (long)gridDim.y * PER) {
+  for (long w = (long)blockIdx.x * PER + threadIdx.x / LANES; w < rows; w += (long)gridDim.x * PER) {
     const bool isv = w & 1;
     const int h = (int)((w >> 1) % c.Hkv), i = (int)((w >> 1) / c.Hkv);
     const long at = kv_slot(c, r, b, h, s.pos + i);
@@ -257,7 +254,7 @@ extern "C" int qvex_paged_append(const qvex_kv_pages* pages, const qvex_kv_rows*
   QVEX_CHECK_ARG(k && v && qvex_aligned(k, 2) && qvex_aligned(v, 2), "%s: null or misaligned k or v", fn);
   const int vec = (k_token % 8 | k_head % 8 | v_token % 8 | v_head % 8) == 0 && qvex_aligned(k, 16) && qvex_aligned(v, 16);
   const int per = KV_THREADS / (pages->D / 8);
-  const dim3 grid(rows->B, kv_grid(((long)r.L * c.Hkv * 2 + per - 1) / per, rows->B));
+  const dim3 grid(kv_grid(((long)r.L * c.Hkv * 2 + per - 1) / per, rows->B), rows->B);
   KV_DISPATCH(paged_append_kernel, pages->format, pages->D, grid, (hipStream_t)stream, c, r, k, k_token, k_head, v,
               v_token, v_head, vec);
   QVEX_CHECK_LAUNCH(fn);
@@ -283,7 +280,7 @@ extern "C" int qvex_paged_qk_rope(const qvex_kv_pages* pages, const qvex_kv_rows
                  "%s: q_out must be 16-byte aligned, freqs 8-byte", fn);
   const int vec = p_stride % 8 == 0 && qvex_aligned(proj, 16) && qvex_aligned(q_norm, 16) && qvex_aligned(k_norm, 16);
   const int per = KV_THREADS / (D / 8);
-  const dim3 grid(rows->B, kv_grid((long)r.L * ((Hq + 2 * c.Hkv + per - 1) / per), rows->B));
+  const dim3 grid(kv_grid((long)r.L * ((Hq + 2 * c.Hkv + per - 1) / per), rows->B), rows->B);
   KV_DISPATCH(paged_qk_rope_kernel, pages->format, D, grid, (hipStream_t)stream, c, r, proj, p_stride, q_norm, k_norm,
               Hq, rot_dim, freqs, eps, q_out, vec);
   QVEX_CHECK_LAUNCH(fn);
@@ -311,7 +308,7 @@ extern "C" int qvex_paged_read(const qvex_kv_pages* pages, const qvex_kv_rows* r
   QVEX_CHECK_ARG(k_out && v_out && qvex_aligned(k_out, 16) && qvex_aligned(v_out, 16),
                  "%s: the outputs must be 16-byte aligned, not null", fn);
   const int per = KV_THREADS / (pages->D / 8);
-  const dim3 grid(rows->B, kv_grid(((long)r.L * c.Hkv * 2 + per - 1) / per, rows->B));
+  const dim3 grid(kv_grid(((long)r.L * c.Hkv * 2 + per - 1) / per, rows->B), rows->B);
   const auto go = pages->D == 256 ? (pages->format == QVEX_KV_BF16   ? &launch_read<QVEX_KV_BF16, 32>
                                      : pages->format == QVEX_KV_INT8 ? &launch_read<QVEX_KV_INT8, 32>
                                                                      : &launch_read<QVEX_KV_FP8, 32>)
