@@ -16,6 +16,10 @@
 // So K, V and P never leave their lanes, and a lane owns one q row. Codes are exact in
 // bf16: K's scale multiplies the score, V's the weight. P goes into the second product
 // as two bf16 terms (16 bits of it), so the output's own rounding is the one that shows.
+//
+// 16 query and 4 kv heads of 256, int8: 64 sequences of one row at up to 8192 keys read 618 MB in 130 to 136 us
+// (4.5 TB/s; a plain read reaches 6.2): the CUs that hold the longest sequences end last. One row at
+// 4096 keys 6 us and 3.6 of merging, four at 7001 (fp8) 10 and 4: two round trips of memory and two launches.
 #include "paged_attn.h"
 
 namespace {
