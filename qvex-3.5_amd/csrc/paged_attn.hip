@@ -421,7 +421,22 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
     // records cost more than the second step: 4 rows at 7001 keys 16 | 14)
     const long blocks = std::max(std::min(B * tiles, full) * Hkv, 1L);
     const long want = p->chunk || L <= 8 ? 256 : 768;             // many row tiles of unequal lengths
-    const long n = std::min(std::max(want / blocks, 1L), steps), least = !p->chunk && most > 8 && steps > 16 ? 2 : 1;
+    const long least = !p->chunk && most > 8 && steps > 16 ? 2 : 1;
+    long n = std::min(std::max(want / blocks, 1L), steps);
+    if (!p->chunk && L <= 8) {
+      // more of them, of 8 steps at least, where that leaves a tenth of the CUs' rounds empty (us, as many as
+      // fit once | so, sequences of unequal | of equal lengths: 48 x 8192 keys 113, 93 | 140, 150; 80 x 3000 76, 63 | 113,
+      // 103; 96 x 4096 119, 109 | 152, 152; 24 x 8192 keys of 8 heads of 128 67, 56 | 78, 79)
+      double best = 0.0;
+      for (long x = n, end = std::max(n, steps / 8); x <= end; ++x) {
+        const double busy = (double)(x * blocks) / ((x * blocks + want - 1) / want * want);
+        if (busy > best + 1e-9) {
+          best = busy;
+          n = x;
+        }
+        if (busy >= 0.9) break;
+      }
+    }
     kps = (int)std::max((steps + n - 1) / n, least) * PA_STEP;
   }
   p->tiles = (int)std::min(tiles, 65535L);   // of a grid
