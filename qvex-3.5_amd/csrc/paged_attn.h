@@ -24,8 +24,9 @@ struct PaArgs {
   const uint16_t* gate;
   long g_token, g_head;
   uint16_t* out;
-  float* ws;                           // O [T * Hq][nsplit][D], then (m, l) [T * Hq][nsplit]
-  int Hq, kps, nsplit, vec;
+  float* ws;                           // O [records][D], then (m, l) [records]
+  size_t records;                      // [T * Hq][nsplit], or of shares [Hkv][shares + B][PA_ROWS]
+  int Hq, kps, nsplit, vec, B, shares;
   float c2;                            // scale * log2(e): scores in base 2
 };
 
@@ -34,7 +35,7 @@ __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((pa_f32x2{lo, hi}), pa_bf16x2));
 }
 __device__ __forceinline__ float2* pa_ml(const PaArgs& a, int D) {
-  return reinterpret_cast<float2*>(a.ws + (size_t)a.r.T * a.Hq * a.nsplit * D);
+  return reinterpret_cast<float2*>(a.ws + a.records * D);
 }
 
 // A uniform word of the block table: a scalar load.
@@ -70,6 +71,21 @@ struct PaBlock {
     kh = a.r.cu ? pair - b * heads : pair;
   }
 };
+
+// Shares: the 128-key steps of all sequences' first tiles, one after another, cut into `shares` equal runs, one
+// per block of a kv head. Run i's part of sequence b leaves record i + b: every further part moves one of the two on.
+__device__ __forceinline__ int pa_steps(const PaArgs& a, int b, int GQ) {
+  const KvSeq s(a.r, b);
+  const int keys = min(s.pos + min(s.n, (PA_ROWS - 1) / GQ + 1), a.r.width << a.c.shift);
+  if (s.n == 0) return 0;
+  // a sequence of more rows than a tile has a first step in any case: its block takes the other tiles too
+  return max((max(keys, 0) + PA_STEP - 1) / PA_STEP, s.n * GQ > PA_ROWS ? 1 : 0);
+}
+__device__ __forceinline__ int pa_wave_sum(int x) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m, 64);
+  return __builtin_amdgcn_readfirstlane(x);
+}
 
 inline dim3 pa_grid(const PaArgs& a, int B, int tiles) {
   return a.r.cu ? dim3(a.c.Hkv * B, tiles, a.nsplit) : dim3(a.c.Hkv * tiles, B, a.nsplit);

@@ -18,8 +18,9 @@
 // as two bf16 terms (16 bits of it), so the output's own rounding is the one that shows.
 //
 // 16 query and 4 kv heads of 256, int8: 64 sequences of one row at up to 8192 keys read 618 MB in 130 to 136 us
-// (4.5 TB/s; a plain read reaches 6.2): the CUs that hold the longest sequences end last. One row at
-// 4096 keys 6 us and 3.6 of merging, four at 7001 (fp8) 10 and 4: two round trips of memory and two launches.
+// with a block per sequence and head (the CUs of the longest end last), in 120 and 6 of merging in equal runs (4.9
+// TB/s; a plain read reaches 6.2). One row at 4096 keys 6 us and 3.6 of merging, four at 7001 (fp8) 10 and
+// 4: two round trips of memory and two launches.
 #include "paged_attn.h"
 
 namespace {
@@ -28,7 +29,8 @@ namespace {
 // 128, alone until their (m, l, O) are merged in LDS. PIPE (splits of several steps): the next
 // step's K is asked for once the scores have this one's, its V behind the second product (us, 8
 // sequences of up to 8192 keys in int8, one split each: 124 -> 95); a split of one step has no next.
-template <int FMT, int D, bool PIPE>
+// SHARES: one block per (kv head, run of the call's steps), which takes the parts of its run one after another.
+template <int FMT, int D, bool PIPE, bool SHARES>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 #pragma clang fp contract(off)
   constexpr int EB = kv_bytes(FMT), KS = D / 32, KU = D * EB / 64, E = D / 16, VW = E * EB / 4, ROW = D * EB;
@@ -37,27 +39,73 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
   __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int li = lane & 15, lg = lane >> 4;
-  const PaBlock blk(a);
-  const int b = blk.b, kh = blk.kh, split = blockIdx.z, GQ = a.Hq / a.c.Hkv;
-  const KvSeq s(a.r, b);
-  const int cap = a.r.width << a.c.shift, rows = s.n * GQ, mask = (1 << a.c.shift) - 1;
+  const int GQ = a.Hq / a.c.Hkv, cap = a.r.width << a.c.shift, mask = (1 << a.c.shift) - 1, split = blockIdx.z;
+  int b, kh, tile, tiles, k_lo, k_hi = 0;
+  int at = 0, end = 0, before = 0, steps = 0;                     // SHARES: steps of the run, of the sequence in it
+  if constexpr (SHARES) {
+    kh = blockIdx.x % a.c.Hkv;
+    int total = 0;
+    for (int c = 0; c < a.B; c += 64) total += pa_wave_sum(c + lane < a.B ? pa_steps(a, c + lane, GQ) : 0);
+    const int run = (total + a.shares - 1) / a.shares;
+    at = (blockIdx.x / a.c.Hkv) * run;
+    end = min(at + run, total);
+    if (at >= end) return;
+    b = a.B;
+    for (int c = 0; c < a.B; c += 64) {
+      const int mine = c + lane < a.B ? pa_steps(a, c + lane, GQ) : 0;
+      int upto = mine;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const int x = __shfl_up(upto, m, 64);
+        upto += lane >= m ? x : 0;
+      }
+      const uint64_t past = __ballot(before + upto > at);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b = c + l;
+        steps = __builtin_amdgcn_readlane(mine, l);
+        before += __builtin_amdgcn_readlane(upto, l) - steps;
+        break;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (b == a.B) return;                                         // only if positions change under the call
+    tile = 0;
+    tiles = 1;
+    k_lo = (at - before) * PA_STEP;
+  } else {
+    const PaBlock blk(a);
+    b = blk.b;
+    kh = blk.kh;
+    tile = blk.tile;
+    tiles = blk.tiles;
+    k_lo = split * a.kps;
+  }
+  KvSeq s(a.r, b);
+  int rows = s.n * GQ;
   const int32_t* table = a.r.table + b * a.r.stride;
   // the first keys' pages, asked for beside the position (-0.4 us of a small call)
-  const int k_lo = split * a.kps;
   auto page_at = [&](int kb) __attribute__((always_inline)) {
     return pa_page(table, min(kb >> a.c.shift, a.r.width - 1));
   };
-  const int first0 = page_at(k_lo + 32 * wave), first1 = page_at(k_lo + 32 * wave + 16);
+  int first0 = page_at(k_lo + 32 * wave), first1 = page_at(k_lo + 32 * wave + 16);
 
-  for (int tile = blk.tile; tile * PA_ROWS < rows; tile += blk.tiles) {
+  while (SHARES || tile * PA_ROWS < rows) {
     const int row = tile * PA_ROWS + li, last = min(rows, (tile + 1) * PA_ROWS) - 1;
     const bool used = row < rows;
     const int i = used ? row / GQ : 0, g = used ? row - i * GQ : 0;
     const int i_lo = tile * PA_ROWS / GQ, i_hi = last / GQ;       // positions of the tile
     const int rlim = used ? min(s.pos + i, cap - 1) : -1;
     const int keys = min(s.pos + i_hi + 1, cap);                  // that any row sees
-    const int k_hi = split == a.nsplit - 1 ? keys : min(k_lo + a.kps, keys);
-    if (k_lo >= k_hi) continue;                                   // uniform; the merge does not read it
+    if constexpr (SHARES) {
+      k_hi = tile ? keys : min((min(end, before + steps) - before) * PA_STEP, keys);
+    } else {
+      k_hi = split == a.nsplit - 1 ? keys : min(k_lo + a.kps, keys);
+      if (k_lo >= k_hi) {                                         // uniform; the merge does not read it
+        tile += tiles;
+        continue;
+      }
+    }
 
     if (FMT != QVEX_KV_INT8) {
       if (threadIdx.x == 0) odd = 0;
@@ -284,23 +332,45 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
           }
         }
       }
-      if (a.nsplit == 1) {
+      if (SHARES ? tile != 0 : a.nsplit == 1) {
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] *= inv;
         PaGate(a, tok, head, d).store(a, tok, head, d, D, acc);
       } else {
-        const size_t rec = ((size_t)tok * a.Hq + head) * a.nsplit + split;
+        const size_t rec = SHARES ? ((size_t)kh * (a.shares + a.B) + blockIdx.x / a.c.Hkv + b) * PA_ROWS + rr
+                                  : ((size_t)tok * a.Hq + head) * a.nsplit + split;
         *reinterpret_cast<float4*>(a.ws + rec * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         if (d == 0) pa_ml(a, D)[rec] = make_float2(mm, ll);
       }
     }
     __syncthreads();
+    if constexpr (SHARES) {
+      if (at == before && (tile + 1) * PA_ROWS < rows) {          // more rows than L promised: all their keys, here
+        ++tile;
+        k_lo = 0;
+      } else {
+        at = min(end, before + steps);
+        before += steps;
+        steps = 0;
+        while (at < end && steps == 0 && ++b < a.B) steps = pa_steps(a, b, GQ);
+        if (steps == 0) break;
+        s = KvSeq(a.r, b);
+        rows = s.n * GQ;
+        table = a.r.table + b * a.r.stride;
+        tile = 0;
+        k_lo = 0;
+      }
+      first0 = page_at(k_lo + 32 * wave);
+      first1 = page_at(k_lo + 32 * wave + 16);
+    } else {
+      tile += tiles;
+    }
   }
 
   // rows of sequences without a visible key (a negative position): nobody else writes them
-  if (a.nsplit == 1 && s.pos < 0) {
-    for (int w = blk.tile; w < s.n && s.pos + w < 0; w += blk.tiles)
+  if (!SHARES && a.nsplit == 1 && s.pos < 0) {
+    for (int w = PaBlock(a).tile; w < s.n && s.pos + w < 0; w += tiles)
       for (int x = threadIdx.x; x < GQ * D; x += 256) a.out[((size_t)(s.first + w) * a.Hq + kh * GQ) * D + x] = 0;
   }
 }
@@ -312,13 +382,20 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 // 8 x 64 at 1000 (8.7M) 47 | 39, at 4000 (33M) 111 | 72, 512 at 4000 (37M) 119 | 75; of 128, 4 and 2
 // heads: 512 at 4000 (9.2M) 33 | 30, 12 x 100 at 1000 (5.3M) 24 | 24, 8 x 200 at 4000 (27M) 67 | 50.
 constexpr long PA_CHUNK_MIN = 64;
+// Many sequences of one tile and of long contexts are cut into equal runs of steps, one per CU (two of 128 dims), in
+// place of equal splits of each: a sequence far below max_keys leaves no CU idle, for a search in
+// the positions and a second launch (4 us), and 2 us for each end of a sequence inside a run. us, splits | runs, lengths
+// 1/8 .. 1 of max_keys | all of them max_keys, 16 and 4 heads of 256: int8 24 x 8192 55, 50 | 78, 80; 40 x 2 rows at
+// 5000 60, 50 | 85, 85; 64 x 8192 131, 121 | 186, 194; bf16 64 x 8192 258, 223 | 360, 366; 16 x 8192 (64 tiles, int8)
+// 35, 38 | 49, 53; 128 x 2000 (16 steps) 64, 71 | 99, 109; 8 heads of 128, int8: 32 x 8192 71, 56 | 95, 103.
+constexpr int PA_SHARE_SEQS = 255;     // times 2^23 steps of a sequence: below 2^31
 constexpr double PA_CHUNK_WORK = 5e6 * 256;
 
 // A row's records merged; D / 4 lanes hold the row, four dims each, eight records requested
 // at a time. WIDE: a block per row, whose groups of lanes take every 256 / (D / 4)-th record and
 // are then merged in their order: few rows of many records are otherwise a chain of round trips
 // (us, 16 rows of 33 records 10.4 -> 4.1, 64 of 28 -> 5.0; many rows of few records need the lanes).
-template <int D, bool WIDE>
+template <int D, bool WIDE, bool SHARES>
 __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
 #pragma clang fp contract(off)
   constexpr int LANES = D / 4, PER = 256 / LANES, BATCH = 8, STEP = WIDE ? PER : 1;
@@ -328,10 +405,34 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
   const KvSeq s(a.r, b);
   const int cap = a.r.width << a.c.shift;
   const long rows = (long)s.n * a.Hq;
+  // SHARES: the runs that have steps of the sequence, run0 .. run0 + runs - 1
+  const int GQ = a.Hq / a.c.Hkv;
+  int run0 = 0, runs = 0;
+  if constexpr (SHARES) {
+    const int lane = threadIdx.x & 63;
+    int total = 0, before = 0, mine = 0;
+    for (int c = 0; c < a.B; c += 64) {
+      const int x = c + lane < a.B ? pa_steps(a, c + lane, GQ) : 0;
+      total += x;
+      before += c + lane < b ? x : 0;
+      mine += c + lane == b ? x : 0;
+    }
+    total = pa_wave_sum(total);
+    before = pa_wave_sum(before);
+    mine = pa_wave_sum(mine);
+    const int run = (total + a.shares - 1) / a.shares;
+    if (mine) {
+      run0 = before / run;
+      runs = (before + mine - 1) / run + 1 - run0;
+    }
+  }
   const int each = WIDE ? 1 : PER;
   for (long w = (long)blockIdx.x * each + (WIDE ? 0 : sub); w < rows; w += (long)gridDim.x * each) {
     const int i = (int)(w / a.Hq), h = (int)(w - (long)i * a.Hq), tok = s.first + i;
-    const size_t rec = ((size_t)tok * a.Hq + h) * a.nsplit;
+    if (SHARES && i * GQ + h % GQ >= PA_ROWS) continue;           // its tile's block has written it
+    const size_t rec = SHARES ? ((size_t)(h / GQ) * (a.shares + a.B) + run0 + b) * PA_ROWS + (i * GQ + h % GQ)
+                              : ((size_t)tok * a.Hq + h) * a.nsplit;
+    constexpr int GAP = SHARES ? PA_ROWS : 1;                     // from a row's record to its next
     const float2* mls = pa_ml(a, D) + rec;
     const float* os = a.ws + rec * D + d;
     float m = PA_NONE, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -342,16 +443,16 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
 #pragma unroll
       for (int x = 0; x < BATCH; ++x) {
         const int at = min(s0 + x * STEP, n - 1);
-        ml[x] = mls[at];
-        ov[x] = *reinterpret_cast<const float4*>(os + (size_t)at * D);
+        ml[x] = mls[at * GAP];
+        ov[x] = *reinterpret_cast<const float4*>(os + (size_t)at * (GAP * D));
       }
     };
-    ask(WIDE ? sub : 0, a.nsplit);
+    if (!SHARES) ask(WIDE ? sub : 0, a.nsplit);
     const PaGate gate(a, tok, h, d);
     const int keys = min(s.pos + i + 1, cap);
-    const int act = keys <= 0 ? 0 : min((keys - 1) / a.kps + 1, a.nsplit);
+    const int act = SHARES ? runs : keys <= 0 ? 0 : min((keys - 1) / a.kps + 1, a.nsplit);
     for (int s0 = WIDE ? sub : 0; s0 < act; s0 += BATCH * STEP) {
-      if (s0 >= BATCH * STEP) ask(s0, act);
+      if (SHARES || s0 >= BATCH * STEP) ask(s0, act);
 #pragma unroll
       for (int x = 0; x < BATCH; ++x) {
         if (s0 + x * STEP >= act) break;
@@ -399,6 +500,8 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
 struct PaPlan {
   bool chunk;                          // paged_chunk.hip's form
   int tiles, kps, nsplit;              // row tiles of the longest sequence; keys per split; splits
+  int shares;                          // or, in place of splits, runs of steps of all sequences
+  uint64_t records;
   uint64_t bytes;
 };
 
@@ -414,7 +517,8 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
   // where L says little of a sequence (every row of the call may be one's), few of B * tiles have rows: the blocks
   // of the longest sequence then take several
   const long tiles = std::min((most + per - 1) / per, std::max(4 * full, 4096L) / B + 1);
-  if (kps == 0) {
+  const bool chosen = kps == 0;
+  if (chosen) {
     // as many splits as give each CU a block (us, int8, 256-dim heads, blocks of one split | n splits: 16
     // x 2000 keys (64 blocks) 28 | 4: 18 | 16: 22; 8 x 4 rows at 4096 (32) 54 | 8: 21 | 33: 30; 64 x 4600 (256) 112
     // | 2: 112 | 36: 154), of two steps at least where a tile is more than half full (its
@@ -424,9 +528,9 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
     const long least = !p->chunk && most > 8 && steps > 16 ? 2 : 1;
     long n = std::min(std::max(want / blocks, 1L), steps);
     if (!p->chunk && L <= 8) {
-      // more of them, of 8 steps at least, where that leaves a tenth of the CUs' rounds empty (us, as many as
-      // fit once | so, sequences of unequal | of equal lengths: 48 x 8192 keys 113, 93 | 140, 150; 80 x 3000 76, 63 | 113,
-      // 103; 96 x 4096 119, 109 | 152, 152; 24 x 8192 keys of 8 heads of 128 67, 56 | 78, 79)
+      // more of them, of 8 steps at least, where these leave a tenth of the CUs' rounds empty (us, as many as
+      // fit once, so, sequences of unequal | of equal lengths: 24 x 8 rows at 8192 keys int8 104, 90 | 117, 133, bf16
+      // 203, 162 | 230, 241; 40 x 8 at 3000 int8 71, 70 | 97, 91, bf16 139, 117 | 179, 159)
       double best = 0.0;
       for (long x = n, end = std::max(n, steps / 8); x <= end; ++x) {
         const double busy = (double)(x * blocks) / ((x * blocks + want - 1) / want * want);
@@ -442,7 +546,14 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
   p->tiles = (int)std::min(tiles, 65535L);   // of a grid
   p->kps = kps;
   p->nsplit = (max_keys - 1) / kps + 1;
-  p->bytes = p->nsplit == 1 ? 0 : (uint64_t)T * Hq * p->nsplit * (D + 2) * sizeof(float);
+  p->shares = 0;
+  p->records = p->nsplit == 1 ? 0 : (uint64_t)T * Hq * p->nsplit;
+  if (chosen && !p->chunk && most <= PA_ROWS && B >= 2 && B <= PA_SHARE_SEQS && (long)B * Hkv >= 96 && steps >= 24) {
+    p->shares = (int)std::max((D == 128 ? 512 : 256) / Hkv, 1);
+    p->records = (uint64_t)Hkv * (p->shares + B) * PA_ROWS;
+    p->nsplit = 1;
+  }
+  p->bytes = p->records * (D + 2) * sizeof(float);
   return true;
 }
 
@@ -451,8 +562,10 @@ void launch_attn(dim3 grid, hipStream_t st, const PaArgs& a) {
   constexpr bool FITS = FMT != QVEX_KV_BF16 || D == 128;         // 16 KB of K and of V per wave leave no registers over
   // many rows: other tiles' waves hide the loads, and fewer registers are worth more (us, two rows' tiles or more, with |
   // without: 12 x 200 rows at 1500 keys 27.9 | 26.8; 2 x 64 at 1000 25.0 | 23.6; 16 x 12 at 2000 39.4 | 38.3)
-  if (FITS && a.kps > PA_STEP && a.r.L <= 8) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, FITS>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false>), grid, dim3(256), 0, st, a);
+  if (a.shares) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, FITS, true>), grid, dim3(256), 0, st, a);
+  else if (FITS && a.kps > PA_STEP && a.r.L <= 8)
+    hipLaunchKernelGGL((paged_attn_kernel<FMT, D, FITS, false>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false, false>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -494,10 +607,13 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
   a.Hq = Hq;
   a.kps = p.kps;
   a.nsplit = p.nsplit;
+  a.records = p.records;
+  a.B = B;
+  a.shares = p.shares;
   a.vec = (q_token % 8 | q_head % 8) == 0 && qvex_aligned(q, 16);
   a.c2 = fmaxf(scale * 1.44269504088896340736f, 1e-37f);       // a masked score stays -inf at a scale of 0 too
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid = pa_grid(a, B, p.tiles);
+  const dim3 grid = p.shares ? dim3(a.c.Hkv * p.shares) : pa_grid(a, B, p.tiles);
   const int f = pages->format;
   const auto go = D == 256 ? (f == QVEX_KV_BF16   ? &launch_attn<QVEX_KV_BF16, 256>
                               : f == QVEX_KV_INT8 ? &launch_attn<QVEX_KV_INT8, 256>
@@ -508,14 +624,15 @@ extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_ro
   if (p.chunk) qvex::paged_chunk_attention(&a, f, D, p.tiles, B, stream);
   else go(grid, st, a);
   QVEX_CHECK_LAUNCH(fn);
-  if (p.nsplit > 1) {
+  if (p.nsplit > 1 || p.shares) {
     // wide by the rows of a sequence alone, so that calls of up to 8 give a row the same bits
-    const bool wide = a.r.L <= 8;
+    const bool wide = a.r.L <= 8 || p.shares;
     const int per = wide ? 1 : 256 / (D / 4);
     const long most = (8192 + B - 1) / B, want = ((long)a.r.L * Hq + per - 1) / per;
     const dim3 mgrid((unsigned)std::min(want, most), B);
-    const auto merge = D == 256 ? (wide ? &paged_attn_merge_kernel<256, true> : &paged_attn_merge_kernel<256, false>)
-                                : (wide ? &paged_attn_merge_kernel<128, true> : &paged_attn_merge_kernel<128, false>);
+    const auto merge = p.shares ? (D == 256 ? &paged_attn_merge_kernel<256, true, true> : &paged_attn_merge_kernel<128, true, true>)
+                       : D == 256 ? (wide ? &paged_attn_merge_kernel<256, true, false> : &paged_attn_merge_kernel<256, false, false>)
+                                  : (wide ? &paged_attn_merge_kernel<128, true, false> : &paged_attn_merge_kernel<128, false, false>);
     hipLaunchKernelGGL(merge, mgrid, dim3(256), 0, st, a);
     QVEX_CHECK_LAUNCH("qvex_paged_attention/merge");
   }

@@ -219,6 +219,15 @@ def test_pool_grows_and_keeps_its_pages(fmt):
         assert torch.equal(a[:2], b)
 
 
+def test_workspace_of_many_long_contexts():
+    """Runs of steps: a record of a tile for each of the runs and sequences of a kv head."""
+    f = _C.lib().qvex_paged_attention_workspace_bytes
+    assert f(64, 1, 64, 16, 4, 256, 8192, 0) == 4 * (64 + 64) * 16 * 258 * 4
+    assert f(30, 2, 60, 32, 8, 128, 8192, 0) == 8 * (64 + 30) * 16 * 130 * 4
+    assert f(64, 1, 64, 16, 4, 256, 8192, 8192 + 128) == 0          # a split length given: its splits
+    assert f(64, 1, 64, 16, 4, 256, 128, 0) == 0
+
+
 def test_workspace_of_a_call_with_and_without_row_offsets():
     """max_rows left out: enough for T / B rows each and for all of them in one sequence."""
     pages = paged.KVPages.alloc(64, 4, 256, "int8", 64, "cpu")

@@ -290,6 +290,54 @@ def test_attention_of_unequal_sequences(dev, fmt, D, Hq, n_kv, page, lens, wide,
     check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, wide=wide, max_rows=max(lens) if bound else None)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,Hq,n_kv,page,lens,pos,max_rows", [
+    (256, 8, 4, 16, [1] * 24, [0, 700, 5, 127, 128, 300] * 4, 1),
+    (128, 4, 2, 32, [1, 2, 0, 4] * 12, [0, 130, 50, 14, -1, -3, 400, 255] * 6, 4),
+    (128, 8, 8, 64, [1] * 100, list(range(0, 300, 3)), 1),          # two rounds of the search
+    (256, 16, 4, 64, [4] + [1] * 23, [900] + [0] * 23, 4),          # one sequence has nearly every step
+    (128, 4, 2, 16, [1] * 20 + [23] + [1] * 30 + [9], [40] * 20 + [-6] + [60] * 30 + [200], 1),   # more rows than max_rows
+    (128, 24, 8, 1024, [2] * 13, [0, -2, 1] * 4 + [1500], 2),
+])
+def test_attention_of_many_long_contexts(dev, fmt, D, Hq, n_kv, page, lens, pos, max_rows):
+    """A bound on the keys far above them: the steps of all sequences in equal runs."""
+    check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, gate=True, wide=True, max_rows=max_rows)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_graph_of_many_long_contexts(dev, fmt):
+    """Replays at new positions, beside eager calls, and the same bits whenever it is called."""
+    D, Hq, n_kv, page, B, W = 256, 8, 4, 64, 30, 64
+    pages = paged.KVPages.alloc(B * W, n_kv, D, fmt, page, dev)
+    for x in pages.tensors():
+        if x.dtype == torch.float32:
+            x.copy_(0.01 + torch.rand(x.shape, generator=gen(41)))
+        elif fmt == "bf16":
+            x.copy_(torch.randn(x.shape, generator=gen(42)))
+        else:
+            x.view(torch.uint8).copy_(torch.randint(0, 100, x.shape, generator=gen(43), dtype=torch.uint8))
+    table = torch.randperm(B * W, generator=gen(44)).to(torch.int32).view(B, W).to(dev)
+    q = torch.randn((B, Hq, D), generator=gen(45)).to(BF16).to(dev)
+    pos = torch.randint(0, W * page, (B,), generator=gen(46)).to(torch.int32).to(dev)
+    want = paged.attention(pages, q, table, pos)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = paged.attention(pages, q, table, pos)
+    torch.cuda.current_stream().wait_stream(s)
+    for i in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(paged.attention(pages, q, table, pos), want)
+        pos.copy_(torch.randint(-1, W * page, (B,), generator=gen(50 + i)))
+        one = paged.attention(pages, q[7:8], table[7:8], pos[7:8])
+        want = paged.attention(pages, q, table, pos)
+        assert torch.allclose(one[0].float(), want[7].float(), rtol=2.0 ** -6, atol=2.0 ** -6 * float(one.abs().max()))
+
+
 def test_append_read_and_input_stage_of_unequal_sequences(dev):
     """Every row of a batch of one long and many short sequences, as in a call of its own."""
     D, Hq, n_kv, page, lens = 128, 4, 2, 16, [300] + [1, 0, 3] * 30 + [64]
