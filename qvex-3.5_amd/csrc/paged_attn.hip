@@ -376,8 +376,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 }
 
 // A call of more than 8 rows per sequence takes the chunk form (paged_chunk.hip) if a sequence's
-// rows of a kv head fill half a block (a quarter on average, whatever L allows) and (query, key) pairs * D are worth its start and end,
-// 8 us against 3. us, this form | that one, int8, 16 query and 4 kv heads of 256 (pairs = T * Hq *
+// rows of a kv head fill half a block (a quarter on average, whatever L allows) and (query, key) pairs
+// * D are worth its start and end, 8 us against 3. us, this form | that one, int8, 16 query and 4 kv heads of 256 (pairs = T * Hq *
 // max_keys): 64 positions at 1000 keys (1.1M) 23 | 24, at 4000 (4.2M) 34 | 33, 512 at 0 (4.2M) 30 | 27,
 // 8 x 64 at 1000 (8.7M) 47 | 39, at 4000 (33M) 111 | 72, 512 at 4000 (37M) 119 | 75; of 128, 4 and 2
 // heads: 512 at 4000 (9.2M) 33 | 30, 12 x 100 at 1000 (5.3M) 24 | 24, 8 x 200 at 4000 (27M) 67 | 50.
