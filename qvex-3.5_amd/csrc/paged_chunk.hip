@@ -23,7 +23,8 @@
 // other vector, 180 scalar and 90 LDS instructions, of which codes to bf16 and their way to LDS are
 // a quarter. Two waves per SIMD that share 32 rows (each one key tile's scores, half the dims of O, weights
 // exchanged in LDS) measured us, int8 | bf16 after 16384 keys | bf16 after 3584: 171 | 168 | 65, this
-// 185 | 171 | 62 (merge included).
+// 185 | 171 | 62 (merge included). A taken branch costs a lone wave some 200 cycles (rescaling O under a branch per
+// tile of it 294 us against 189), so what is rare lies behind the loop (fp8 187 -> 180).
 #include "paged_attn.h"
 
 namespace {
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
     // become 0, since 0 times a NaN is none. So does a NaN or an infinity that some rows do not see: the
     // rows that do are marked at the end.
     auto clean = [&](int kb, int ok_all) __attribute__((always_inline)) {
-      if (kb + PC_KEYS <= min(first_lim + 1, k_hi) && ok_all == 15) return;
+      if (__builtin_expect(kb + PC_KEYS <= min(first_lim + 1, k_hi) && ok_all == 15, 1)) return;
       bool any = false;
       if constexpr (EB == 1) {
         const int x = lane & 15;
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
           }
         }
       }
-      if (any) odd = 1;
+      if (__builtin_expect(any, 0)) odd = 1;
     };
     // Pieces of a step's way to LDS, K's and V's
     constexpr int KP = EB == 2 ? KU : 2 * KU, VP = E / 2;
@@ -268,10 +269,11 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
       const bool edge = kb + PC_KEYS > min(w_lim + 1, k_hi) || ok != 15;
       pc_f32x16 sc[2] = {zero, zero};
       u32x4 ring[PC_AHEAD];
+      float wt[16];                                             // a tile's weights
       // the scores of key tile kt, scaled and masked; m moved if they pass it (what has it as its reference follows)
       auto finish = [&](int kt) __attribute__((always_inline)) {
         if constexpr (EB == 1) scale16(sc[kt], ksc[kt]);
-        if (edge) {
+        if (__builtin_expect(edge, 0)) {
           const int lim = min(rlim, k_hi - 1) - kb - 4 * hf;
 #pragma unroll
           for (int x = 0; x < 16; ++x)
@@ -281,7 +283,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
 #pragma unroll
         for (int x = 1; x < 16; ++x) top = fmaxf(top, sc[kt][x]);
         if constexpr (EB == 2) top *= a.c2;
-        if (__any(top - m > PA_SLACK)) {
+        if (__builtin_expect(__any(top - m > PA_SLACK), 0)) {
           const float x = fmaxf(top, __shfl_xor(top, 32, 64));  // of the row, in its two lanes
           const float mn = x - m > PA_SLACK ? x : m;
           const float f = __builtin_amdgcn_exp2f(m - mn);
@@ -292,7 +294,9 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
             o[n] *= f;
             __builtin_amdgcn_sched_barrier(0);                  // a tile of O at a time
           }
-          if (kt == 1) sc[0] *= f;
+          if (kt == 1)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) wt[x] *= f;
         }
       };
       // weight x of tile kt, times its value's scale
@@ -301,12 +305,12 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         l += w;
         if constexpr (EB == 1) w *= row_lane_of(vsc[kt], x);
         asm volatile("" : "+v"(w));                             // evaluated here, beside a product
-        sc[kt][x] = w;
+        wt[x] = w;
       };
-      auto packed = [&](int kt, int t) __attribute__((always_inline)) {
+      auto packed = [&](int t) __attribute__((always_inline)) {
         u32x4 p;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = pa_pack(sc[kt][8 * t + 2 * e], sc[kt][8 * t + 2 * e + 1]);
+        for (int e = 0; e < 4; ++e) p[e] = pa_pack(wt[8 * t + 2 * e], wt[8 * t + 2 * e + 1]);
         return p;
       };
 
@@ -332,7 +336,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         __builtin_amdgcn_sched_barrier(0);
       }
       finish(1);
-      u32x4 p0 = packed(0, 0), p1 = packed(0, 1);
+      u32x4 p0 = packed(0), p1 = packed(1);
 #pragma unroll
       for (int y = 0; y < 2 * NT; ++y) {
         const int x = 2 * KS + y;
@@ -343,8 +347,8 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         for (int z = y * 8 / NT; z < (y + 1) * 8 / NT; ++z) weight(1, z);
         __builtin_amdgcn_sched_barrier(0);
       }
-      p0 = packed(1, 0);
-      p1 = packed(1, 1);
+      p0 = packed(0);
+      p1 = packed(1);
       clean(kb + PC_KEYS, ok_next);
 #pragma unroll
       for (int y = 0; y < 2 * NT; ++y) {                        // beside the next step's V
