@@ -18,10 +18,9 @@
 // term would be a third product as long as the two.
 //
 // 16 query and 4 kv heads of 256: 512 positions after 3584 bf16 keys 57 us and 8.6 of merging (500
-// TFLOP/s), after 16384 int8 keys 178 and 8.6 (750). One wave per SIMD holds 32 rows of Q and O in 192
-// registers, and what bounds it is its own issue: a step of 64 keys has 64 products (2048 cycles) and some 570
-// other vector, 180 scalar and 90 LDS instructions, of which codes to bf16 and their way to LDS are
-// a quarter. Two waves per SIMD that share 32 rows (each one key tile's scores, half the dims of O, weights
+// TFLOP/s), after 16384 int8 keys 173 to 185 and 8.6 (760). One wave per SIMD holds 32 rows of Q and O in 192
+// registers, and what bounds it is its own issue: a step of 64 int8 keys has 64 products (2048 cycles) and some
+// 800 other instructions of 4 cycles, of which codes to bf16 and their way to LDS are 300. Two waves per SIMD that share 32 rows (each one key tile's scores, half the dims of O, weights
 // exchanged in LDS) measured us, int8 | bf16 after 16384 keys | bf16 after 3584: 171 | 168 | 65, this
 // 185 | 171 | 62 (merge included). A taken branch costs a lone wave some 200 cycles (rescaling O under a branch per
 // tile of it 294 us against 189), so what is rare lies behind the loop (fp8 187 -> 180).
@@ -91,26 +90,20 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
     uint32_t vraw[4][VW];
     float ksn[2], vsn[2];
     uint32_t s0, s1, s2, s3;                                      // first slots of a step's 16-key groups
-    int g0, g1, g2, g3;                                           // their pages, asked for a step before
-    auto ask = [&](int kb) __attribute__((always_inline)) {
-      g0 = pa_page(table, min(kb >> a.c.shift, a.r.width - 1));
-      g1 = pa_page(table, min((kb + 16) >> a.c.shift, a.r.width - 1));
-      g2 = pa_page(table, min((kb + 32) >> a.c.shift, a.r.width - 1));
-      g3 = pa_page(table, min((kb + 48) >> a.c.shift, a.r.width - 1));
-    };
+    // Lane x finds group x % 4: one load a step before and 20 instructions (us after 16384 keys, int8, 256- | 128-dim
+    // heads: 181 | 219; as scalar code, 80 instructions, 187 | 228)
+    const int x16 = 16 * (lane & 3);
+    int asked;                                                    // the page of the next step's group
+    auto ask = [&](int kb) __attribute__((always_inline)) { asked = table[min((kb + x16) >> a.c.shift, a.r.width - 1)]; };
     auto locate = [&](int kb) __attribute__((always_inline)) {    // returns which of the pages there are
-      int ok_all = 0;
-      auto at = [&](int pg, int x) __attribute__((always_inline)) {
-        const bool ok = pg >= 0 && pg < a.c.n_pages;
-        ok_all |= (ok ? 1 : 0) << x;
-        return (((uint32_t)(ok ? pg : 0) * a.c.Hkv + kh) << a.c.shift) + ((kb + 16 * x) & mask);
-      };
-      s0 = at(g0, 0);
-      s1 = at(g1, 1);
-      s2 = at(g2, 2);
-      s3 = at(g3, 3);
+      const bool ok = asked >= 0 && asked < a.c.n_pages;
+      const uint32_t at = (((uint32_t)(ok ? asked : 0) * a.c.Hkv + kh) << a.c.shift) + ((kb + x16) & mask);
+      s0 = __builtin_amdgcn_readlane(at, 0);
+      s1 = __builtin_amdgcn_readlane(at, 1);
+      s2 = __builtin_amdgcn_readlane(at, 2);
+      s3 = __builtin_amdgcn_readlane(at, 3);
       ask(min(kb + PC_KEYS, k_last));
-      return ok_all;
+      return (int)__ballot(ok) & 15;
     };
     // a lane's scale of key tile kt: key 8 (x / 4) + 4 hf + x % 4 of it, x = lane % 16
     const uint32_t sc_at = 8 * ((lane >> 2) & 1) + 4 * hf + (lane & 3);
