@@ -197,15 +197,11 @@ def prepare(case, seed):
 
 
 def _paged():
-    global _module
-    if _module is None:              # imported once, as a program does
-        sys.path.insert(0, os.path.join(os.getcwd(), "qvex-3.5_amd"))
-        from qvex import paged
-        _module = paged
-    return _module
-
-
-_module = None
+    path = os.path.join(os.getcwd(), "qvex-3.5_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from qvex import paged
+    return paged
 
 
 # ---------------------------------------------------------------- plain forms
