@@ -687,7 +687,9 @@ class Attention:
         self.qkv_proj = QLinear.fuse([p["q_proj"], p["k_proj"], p["v_proj"]])
         self.o_proj = p["o_proj"]
         self.q_norm, self.k_norm = p["q_norm"], p["k_norm"]
-        self._ws = self._freqs = None
+        self._ws = None
+        # of paged caches' rotation; made here, since a layer's first call may be inside a graph capture
+        self._freqs = paged.rope_freqs(cfg.rotary_dim, cfg.rope_theta, self.q_norm.device) if cfg.rotary_dim else None
 
     def _workspace(self, L, cap, kps, device):
         need = int(_C.lib().qvex_attn_workspace_bytes(L, self.n_heads, self.n_kv, self.head_dim, cap, kps))
@@ -699,10 +701,6 @@ class Attention:
         """The rows' attention over a paged cache: the input stage and the append in one launch, then the pages."""
         L, H, D = proj.shape[0], self.n_heads, self.head_dim
         max_keys = cache.capacity if cache.counters.graph_mode else cache.offset + L
-        if self.cfg.rotary_dim and self._freqs is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise _C.QvexError("the rotation's frequencies are made by an eager step, not inside a graph capture")
-            self._freqs = paged.rope_freqs(self.cfg.rotary_dim, self.cfg.rope_theta, proj.device)
         pages = cache.pages
         q = paged.attn_qk_rope(pages, proj, self.q_norm, self.k_norm, cache.table, cache.pos, self._freqs,
                                float(self.cfg.rms_norm_eps))

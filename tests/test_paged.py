@@ -312,3 +312,18 @@ def test_clone_of_layer_caches_shares_one_table_of_counters():
     twin[0].offset = 131
     assert caches[0].offset == 130 and twin[1].offset == 130
     assert twin[0].pos.data_ptr() == twin.counters.ptr(0) and caches[1].pos.data_ptr() == counters.ptr(1)
+
+
+@pytest.mark.parametrize("rotary_dim", [32, 0])
+def test_attention_layer_has_its_frequencies_before_any_call(monkeypatch, rotary_dim):
+    """A layer's first call may be inside a graph capture, where none can be made."""
+    from qvex.model import Attention, Config, QLinear
+    monkeypatch.setattr(QLinear, "fuse", staticmethod(lambda layers: None))
+    cfg = Config.tiny()
+    cfg.rotary_dim = rotary_dim
+    w = torch.ones(cfg.head_dim, dtype=BF16)
+    layer = Attention(cfg, {**dict.fromkeys(("q_proj", "k_proj", "v_proj", "o_proj")), "q_norm": w, "k_norm": w})
+    if rotary_dim:
+        assert torch.equal(layer._freqs, paged.rope_freqs(32, cfg.rope_theta, "cpu"))
+    else:
+        assert layer._freqs is None

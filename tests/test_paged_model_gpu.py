@@ -195,3 +195,13 @@ def test_bf16_pages_and_dense_caches_agree(tiny):
         outs.append([model(ids_of(n, V, n), cache, last_only=False).float() for n in (130, 40, 4, 1)])
     for a, b in zip(*outs):
         assert float((a - b).abs().max()) <= 2 * 2.0 ** -7 * float(a.abs().max())
+
+
+@pytest.mark.parametrize("fmt", [None, *FORMATS])
+def test_one_token_prompt_on_a_fresh_head(dev, fmt):
+    """The first call of the MTP head's attention is inside the capture of the cycle (a prompt of one token leaves it no pair)."""
+    model = random_model(Config.tiny(layers=4, vocab=2048), seed=7, device=dev, max_context=256)
+    params = SamplingParams(temperature=0.0, top_k=0, top_p=1.0, max_tokens=12)
+    on = generate(model, [17], params, random_mtp(model, seed=8), "on", kv=fmt)
+    assert on.stats["mtp_graph_cycles"] == on.stats["mtp_cycles"] > 0
+    assert on.tokens == generate(model, [17], params, None, "off", kv=fmt).tokens and len(on.tokens) == 12
