@@ -331,7 +331,14 @@ class GraphedMTPCycle:
         d.mtp_cache.counters.graph_mode = True
         self.released = False
         old = self.graph
-        self.graph = self._capture(self.out, pool=None if old is None else old.pool(), done=self.done)
+        try:
+            self.graph = self._capture(self.out, pool=None if old is None else old.pool(), done=self.done)
+        except BaseException:
+            # nothing has run: the decoder still has its pairs and feed, the draw is given back
+            d.cache.counters.graph_mode = d.mtp_cache.counters.graph_mode = False
+            d.sampler.counter(self.u_buf.device).sub_(1)
+            self.released = True
+            raise
         self._pipe = None
         return self
 
@@ -350,11 +357,11 @@ class GraphedMTPCycle:
                 self._body(out, done)
         finally:
             d.cache.counters.capturing = d.mtp_cache.counters.capturing = False
-        d.cache.counters.host[:] = host_main
-        d.mtp_cache.counters.host[:] = host_mtp
-        for c, w in zip(d.cache, widths):
-            if w is not None:
-                c.last_width = w
+            d.cache.counters.host[:] = host_main
+            d.mtp_cache.counters.host[:] = host_mtp
+            for c, w in zip(d.cache, widths):
+                if w is not None:
+                    c.last_width = w
         return g
 
     def _commit(self, counters, n_ptr, extra):

@@ -73,3 +73,49 @@ def test_recurrent_rollback_bounded_and_clone_independent():
     assert float(rc.ssm_ring.abs().sum()) == 0.0 and float(twin[1].k.abs().sum()) == 0.0
     assert twin[0].counters is twin[1].counters and twin.counters is not counters
     assert np.array_equal(counters.host, np.array([8, 0], np.int32))
+
+
+def test_a_capture_that_fails_gives_the_caches_back(monkeypatch):
+    """GraphedMTPCycle.attach whose capture raises: the decoder, its caches and the draws are as before, and may go on."""
+    import contextlib
+    from types import SimpleNamespace
+
+    from qvex.speculative import GraphedMTPCycle
+
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: None)
+    monkeypatch.setattr(torch.cuda, "graph", lambda g, pool=None: contextlib.nullcontext())
+    draws = torch.zeros(1, dtype=torch.int64)
+    sampler = SimpleNamespace(draw_into=lambda u: draws.add_(1), prepare_accept=lambda k, dev: None, counter=lambda dev: draws)
+    caches = [KVCache(None, 0, n_kv=1, head_dim=64, capacity=256, device="cpu") for _ in range(2)]
+    for c in caches:
+        c.offset = 7
+    caches[0].last_width = 1
+    dec = SimpleNamespace(pend_h=[torch.ones(1, 1, 4)], pend_ids=[torch.ones(1, 1, dtype=torch.int32)],
+                          feed=torch.tensor([5], dtype=torch.int32), sampler=sampler,
+                          model=SimpleNamespace(cfg=SimpleNamespace(rotary_dim=0, rope_theta=1e6)),
+                          cache=LayerCaches(caches[:1], caches[0].counters), mtp_cache=caches[1])
+    g = GraphedMTPCycle.__new__(GraphedMTPCycle)
+    g.dec, g.k, g.released, g.graph, g._pipe, g._kv = dec, 3, True, None, None, caches[:1]
+    g.pend_h, g.pend_ids = torch.zeros(1, 4, 4), torch.zeros(1, 4, dtype=torch.int32)
+    g.n_prev, g.feed, g.ids = (torch.zeros(s, dtype=torch.int32) for s in (1, 1, (1, 4)))
+    g.u_buf, g.out, g.done = torch.zeros(4), None, None
+
+    def body(out, done):
+        for c in caches:
+            assert c.counters.graph_mode and c.counters.capturing
+            c.offset += 4
+        caches[0].last_width = 4
+        raise _C.QvexError("in the capture")
+
+    g._body = body
+    for _ in range(2):
+        with pytest.raises(_C.QvexError, match="in the capture"):
+            g.attach()
+        assert g.released and int(draws) == 0 and caches[0].last_width == 1
+        for c in caches:
+            assert not c.counters.graph_mode and not c.counters.capturing and c.offset == 7
+    for c in caches:
+        c.rollback(1)                 # eager control
+    g._body = lambda out, done: None
+    assert g.attach() is g and not g.released and int(draws) == 1 and all(c.counters.graph_mode for c in caches)
