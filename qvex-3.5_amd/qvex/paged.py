@@ -401,18 +401,20 @@ class PagedKVCache:
         self.table[0, :len(self.ids)].copy_(torch.tensor(self.ids, dtype=torch.int32))
 
     def _own(self, at: int) -> None:
-        """The pages from position `at` on become this cache's alone (those behind `offset` are)."""
-        first, changed = at // self.pool.page, False
-        for x in range(first, min(self.offset // self.pool.page + 1, len(self.ids))):
-            j = self.ids[x]
-            if self.pool.holders[j] > 1:
-                self.ids[x] = self.pool.take(1)[0]
-                if x == first and at % self.pool.page:
-                    self.pool.copy(j, self.ids[x])
-                self.pool.give([j])
-                changed = True
-        if changed:
-            self._upload()
+        """The pages from position `at` on become this cache's alone (those behind `offset` are).
+        All of them are taken first: a pool that cannot give them raises with nothing changed."""
+        page, holders = self.pool.page, self.pool.holders
+        first = at // page
+        shared = [x for x in range(first, min(self.offset // page + 1, len(self.ids))) if holders[self.ids[x]] > 1]
+        if not shared:
+            return
+        fresh, old = self.pool.take(len(shared)), [self.ids[x] for x in shared]
+        if shared[0] == first and at % page:
+            self.pool.copy(old[0], fresh[0])
+        for x, j in zip(shared, fresh):
+            self.ids[x] = j
+        self._upload()
+        self.pool.give(old)
 
     def grow(self, min_capacity: int) -> bool:
         """Pages for at least min_capacity positions, in steps of 256 (a HIP graph

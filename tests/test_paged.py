@@ -327,3 +327,57 @@ def test_attention_layer_has_its_frequencies_before_any_call(monkeypatch, rotary
         assert torch.equal(layer._freqs, paged.rope_freqs(32, cfg.rope_theta, "cpu"))
     else:
         assert layer._freqs is None
+
+
+def shared_pair(free, growable=False):
+    """A cache at 100 of pages of 16, its clone, and `free` pages left in their pool."""
+    pool = paged.PagePool(32, 2, 128, "int8", 16, "cpu", growable=growable)
+    fill(pool)
+    a = paged.PagedKVCache(pool, capacity=256)
+    a.offset = 100
+    b = a.clone()
+    kept = pool.take(len(pool.free) - free)
+    fill(pool)
+    return pool, a, b, kept
+
+
+def state_of(pool, *caches):
+    return (list(pool.holders), sorted(pool.free), [t.clone() for t in pool.pages.tensors()],
+            [(list(c.ids), c.offset, c.table.tolist()) for c in caches])
+
+
+def assert_same(x, y):
+    assert x[0] == y[0] and x[1] == y[1] and x[3] == y[3] and all(torch.equal(s, t) for s, t in zip(x[2], y[2]))
+
+
+@pytest.mark.parametrize("to,free", [(30, 2), (30, 4), (0, 5), (80, 0), (7, 5)])
+def test_a_rollback_without_pages_changes_nothing(to, free):
+    """From 100 back to `to`: pages to // 16 .. 5 are shared, and more of them than are free (page 6 is
+    the cache's own)."""
+    pool, a, b, kept = shared_pair(free)
+    need = 6 - to // 16
+    before = state_of(pool, a, b)
+    with pytest.raises(_C.QvexError, match=f"{free} free pages of 32, {need} are needed"):
+        a.rollback(100 - to)
+    assert_same(before, state_of(pool, a, b))
+    pool.give(kept[:need - free])
+    ids = list(a.ids)
+    a.rollback(100 - to)                      # with enough of them
+    first = to // 16
+    assert a.offset == to and a.ids[:first] == ids[:first] and not set(a.ids[first:6]) & set(b.ids)
+    assert a.table[0, :len(a.ids)].tolist() == a.ids and b.ids == before[3][1][0]
+    if to % 16:
+        for t in pool.pages.tensors():
+            assert torch.equal(t[a.ids[first]], t[b.ids[first]])
+
+
+def test_a_rollback_that_a_captured_cycle_forbids_to_grow_changes_nothing():
+    pool, a, b, _ = shared_pair(1, growable=True)
+    b.counters.graph_mode = True
+    before = state_of(pool, a, b)
+    with pytest.raises(_C.QvexError, match="captured cycle drives"):
+        a.rollback(70)
+    assert_same(before, state_of(pool, a, b))
+    b.counters.graph_mode = False
+    a.rollback(70)
+    assert a.offset == 30 and pool.pages.n_pages > 32 and not set(a.ids[1:]) & set(b.ids)
