@@ -436,7 +436,7 @@ class PagedKVCache:
         c.pos = c.counters.dev[c.index:c.index + 1]
         n = self.offset // self.pool.page
         size = -(-(self.offset + 1) // self.step) * self.step
-        fresh = self.pool.take(-(-size // self.pool.page) - n)
+        c.ids = fresh = self.pool.take(-(-size // self.pool.page) - n)   # given back if what follows raises
         if self.offset % self.pool.page:
             self.pool.copy(self.ids[n], fresh[0])
         self.pool.share(self.ids[:n])

@@ -1,6 +1,7 @@
 """Paged KV cache on the CPU: what the entry points and their front end refuse, before any GPU work."""
 
 import ctypes
+import gc
 
 import pytest
 import torch
@@ -329,9 +330,9 @@ def test_attention_layer_has_its_frequencies_before_any_call(monkeypatch, rotary
         assert layer._freqs is None
 
 
-def shared_pair(free, growable=False):
+def shared_pair(free, growable=False, n_pages=32):
     """A cache at 100 of pages of 16, its clone, and `free` pages left in their pool."""
-    pool = paged.PagePool(32, 2, 128, "int8", 16, "cpu", growable=growable)
+    pool = paged.PagePool(n_pages, 2, 128, "int8", 16, "cpu", growable=growable)
     fill(pool)
     a = paged.PagedKVCache(pool, capacity=256)
     a.offset = 100
@@ -381,3 +382,17 @@ def test_a_rollback_that_a_captured_cycle_forbids_to_grow_changes_nothing():
     b.counters.graph_mode = False
     a.rollback(70)
     assert a.offset == 30 and pool.pages.n_pages > 32 and not set(a.ids[1:]) & set(b.ids)
+
+
+def test_a_clone_that_fails_returns_its_pages(monkeypatch):
+    pool, a, b, _ = shared_pair(14, n_pages=64)
+    before = state_of(pool, a, b)
+
+    def fails(*_):
+        raise MemoryError
+
+    monkeypatch.setattr(pool, "copy", fails)
+    with pytest.raises(MemoryError):
+        a.clone()
+    gc.collect()
+    assert before[0] == pool.holders and before[1] == sorted(pool.free)
