@@ -663,8 +663,8 @@ int qvex_paged_read(const qvex_kv_pages* pages, const qvex_kv_rows* rows, void* 
  * block of a row's split (a multiple of 128), or 0 to choose by the call's size;
  * at one positive value a row's bits do not depend on the other rows of the call,
  * as long as the calls have up to 8 rows per sequence.
- * workspace: qvex_paged_attention_workspace_bytes() of the same arguments,
- * 16-byte aligned (NULL where that is 0); it need not be cleared. */
+ * workspace: qvex_paged_attention_workspace_bytes() of the same arguments, or of
+ * a larger max_keys, 16-byte aligned (NULL where that is 0); it need not be cleared. */
 uint64_t qvex_paged_attention_workspace_bytes(int B, int L, int T, int Hq, int Hkv, int D,
                                               int max_keys, int keys_per_split);
 int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_rows* rows, const uint16_t* q,

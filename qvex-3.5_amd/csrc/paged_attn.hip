@@ -389,6 +389,7 @@ constexpr long PA_CHUNK_MIN = 64;
 // 5000 60, 50 | 85, 85; 64 x 8192 131, 121 | 186, 194; bf16 64 x 8192 258, 223 | 360, 366; 16 x 8192 (64 tiles, int8)
 // 35, 38 | 49, 53; 128 x 2000 (16 steps) 64, 71 | 99, 109; 8 heads of 128, int8: 32 x 8192 71, 56 | 95, 103.
 constexpr int PA_SHARE_SEQS = 255;     // times 2^23 steps of a sequence: below 2^31
+constexpr int PA_SHARE_STEPS = 24;     // of max_keys, at least
 constexpr double PA_CHUNK_WORK = 5e6 * 256;
 
 // A row's records merged; D / 4 lanes hold the row, four dims each, eight records requested
@@ -505,6 +506,41 @@ struct PaPlan {
   uint64_t bytes;
 };
 
+struct PaTiles {
+  long tiles, blocks;                  // row tiles of the longest sequence, blocks with rows
+};
+PaTiles pa_tiles(bool chunk, int B, int L, int T, long GQ, int Hkv) {
+  const int per = chunk ? qvex::PA_CHUNK_ROWS : PA_ROWS;
+  const long most = std::min(L, std::max(T, 1)) * GQ, full = (long)T * GQ / per + B;   // tiles with rows, at most
+  // where L says little of a sequence (every row of the call may be one's), few of B * tiles have rows: the blocks
+  // of the longest sequence then take several
+  const long tiles = std::min((most + per - 1) / per, std::max(4 * full, 4096L) / B + 1);
+  return {tiles, std::max(std::min(B * tiles, full) * Hkv, 1L)};
+}
+
+// As many splits as give each CU a block (us, int8, 256-dim heads, blocks of one split | n splits: 16
+// x 2000 keys (64 blocks) 28 | 4: 18 | 16: 22; 8 x 4 rows at 4096 (32) 54 | 8: 21 | 33: 30; 64 x 4600 (256) 112
+// | 2: 112 | 36: 154). Never fewer for more steps.
+long pa_splits(bool chunk, int L, long blocks, long steps) {
+  const long want = chunk || L <= 8 ? 256 : 768;                  // many row tiles of unequal lengths
+  long n = std::min(std::max(want / blocks, 1L), steps);
+  if (!chunk && L <= 8) {
+    // more of them, of 8 steps at least, where these leave a tenth of the CUs' rounds empty (us, as many as
+    // fit once, so, sequences of unequal | of equal lengths: 24 x 8 rows at 8192 keys int8 104, 90 | 117, 133, bf16
+    // 203, 162 | 230, 241; 40 x 8 at 3000 int8 71, 70 | 97, 91, bf16 139, 117 | 179, 159)
+    double best = 0.0;
+    for (long x = n, end = std::max(n, steps / 8); x <= end; ++x) {
+      const double busy = (double)(x * blocks) / ((x * blocks + want - 1) / want * want);
+      if (busy > best + 1e-9) {
+        best = busy;
+        n = x;
+      }
+      if (busy >= 0.9) break;
+    }
+  }
+  return n;
+}
+
 bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps, PaPlan* p) {
   if (B < 1 || L < 1 || T < 0 || Hkv < 1 || Hq < Hkv || Hq % Hkv || (D != 128 && D != 256) || max_keys < 1 ||
       max_keys > KV_LIMIT || kps < 0 || kps % PA_STEP)
@@ -512,49 +548,47 @@ bool pa_plan(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps,
   const long GQ = Hq / Hkv, most = std::min(L, std::max(T, 1)) * GQ;
   p->chunk = L > 8 && most >= PA_CHUNK_MIN && (double)T * GQ >= 0.5 * PA_CHUNK_MIN * B &&
              (double)T * Hq * max_keys * D >= PA_CHUNK_WORK;
-  const int per = p->chunk ? qvex::PA_CHUNK_ROWS : PA_ROWS;
-  const long full = (long)T * GQ / per + B, steps = (max_keys + PA_STEP - 1) / PA_STEP;   // tiles with rows, at most
-  // where L says little of a sequence (every row of the call may be one's), few of B * tiles have rows: the blocks
-  // of the longest sequence then take several
-  const long tiles = std::min((most + per - 1) / per, std::max(4 * full, 4096L) / B + 1);
+  const long steps = (max_keys + PA_STEP - 1) / PA_STEP;
+  const PaTiles t = pa_tiles(p->chunk, B, L, T, GQ, Hkv);
   const bool chosen = kps == 0;
   if (chosen) {
-    // as many splits as give each CU a block (us, int8, 256-dim heads, blocks of one split | n splits: 16
-    // x 2000 keys (64 blocks) 28 | 4: 18 | 16: 22; 8 x 4 rows at 4096 (32) 54 | 8: 21 | 33: 30; 64 x 4600 (256) 112
-    // | 2: 112 | 36: 154), of two steps at least where a tile is more than half full (its
-    // records cost more than the second step: 4 rows at 7001 keys 16 | 14)
-    const long blocks = std::max(std::min(B * tiles, full) * Hkv, 1L);
-    const long want = p->chunk || L <= 8 ? 256 : 768;             // many row tiles of unequal lengths
+    // two steps at least where a tile is more than half full (its records cost more than the second step: 4
+    // rows at 7001 keys 16 | 14)
     const long least = !p->chunk && most > 8 && steps > 16 ? 2 : 1;
-    long n = std::min(std::max(want / blocks, 1L), steps);
-    if (!p->chunk && L <= 8) {
-      // more of them, of 8 steps at least, where these leave a tenth of the CUs' rounds empty (us, as many as
-      // fit once, so, sequences of unequal | of equal lengths: 24 x 8 rows at 8192 keys int8 104, 90 | 117, 133, bf16
-      // 203, 162 | 230, 241; 40 x 8 at 3000 int8 71, 70 | 97, 91, bf16 139, 117 | 179, 159)
-      double best = 0.0;
-      for (long x = n, end = std::max(n, steps / 8); x <= end; ++x) {
-        const double busy = (double)(x * blocks) / ((x * blocks + want - 1) / want * want);
-        if (busy > best + 1e-9) {
-          best = busy;
-          n = x;
-        }
-        if (busy >= 0.9) break;
-      }
-    }
+    const long n = pa_splits(p->chunk, L, t.blocks, steps);
     kps = (int)std::max((steps + n - 1) / n, least) * PA_STEP;
   }
-  p->tiles = (int)std::min(tiles, 65535L);   // of a grid
+  p->tiles = (int)std::min(t.tiles, 65535L);   // of a grid
   p->kps = kps;
   p->nsplit = (max_keys - 1) / kps + 1;
   p->shares = 0;
   p->records = p->nsplit == 1 ? 0 : (uint64_t)T * Hq * p->nsplit;
-  if (chosen && !p->chunk && most <= PA_ROWS && B >= 2 && B <= PA_SHARE_SEQS && (long)B * Hkv >= 96 && steps >= 24) {
+  if (chosen && !p->chunk && most <= PA_ROWS && B >= 2 && B <= PA_SHARE_SEQS && (long)B * Hkv >= 96 && steps >= PA_SHARE_STEPS) {
     p->shares = (int)std::max((D == 128 ? 512 : 256) / Hkv, 1);
     p->records = (uint64_t)Hkv * (p->shares + B) * PA_ROWS;
     p->nsplit = 1;
   }
   p->bytes = p->records * (D + 2) * sizeof(float);
   return true;
+}
+
+// Bytes that calls of these arguments and of any keys up to max_keys take: splits of whole steps are rounded, so
+// that fewer keys can have more of them (16 query and 4 kv heads of 256, a row: 32 at 8192 keys, 18 at 9000).
+uint64_t pa_most_bytes(int B, int L, int T, int Hq, int Hkv, int D, int max_keys, int kps) {
+  PaPlan p;
+  if (!pa_plan(B, L, T, Hq, Hkv, D, max_keys, kps, &p)) return 0;
+  uint64_t records = p.records;
+  if (kps == 0 && T > 0) {
+    const long steps = (max_keys + PA_STEP - 1) / PA_STEP;
+    const auto more = [&](bool chunk, long most) {
+      const long n = pa_splits(chunk, L, pa_tiles(chunk, B, L, T, Hq / Hkv, Hkv).blocks, std::min(steps, most));
+      if (n > 1) records = std::max(records, (uint64_t)T * Hq * n);
+    };
+    if (p.shares) more(false, PA_SHARE_STEPS - 1);                // the other form's calls are shorter
+    else more(false, p.chunk ? (long)(PA_CHUNK_WORK / ((double)T * Hq * D)) / PA_STEP + 2 : steps);
+    if (p.chunk) more(true, steps);
+  }
+  return records * (D + 2) * sizeof(float);
 }
 
 template <int FMT, int D>
@@ -572,8 +606,7 @@ void launch_attn(dim3 grid, hipStream_t st, const PaArgs& a) {
 
 extern "C" uint64_t qvex_paged_attention_workspace_bytes(int B, int L, int T, int Hq, int Hkv, int D, int max_keys,
                                                          int keys_per_split) {
-  PaPlan p;
-  return pa_plan(B, L, T, Hq, Hkv, D, max_keys, keys_per_split, &p) ? p.bytes : 0;
+  return pa_most_bytes(B, L, T, Hq, Hkv, D, max_keys, keys_per_split);
 }
 
 extern "C" int qvex_paged_attention(const qvex_kv_pages* pages, const qvex_kv_rows* rows, const uint16_t* q,

@@ -396,3 +396,17 @@ def test_a_clone_that_fails_returns_its_pages(monkeypatch):
         a.clone()
     gc.collect()
     assert before[0] == pool.holders and before[1] == sorted(pool.free)
+
+
+@pytest.mark.parametrize("B,L,T,Hq,Hkv,D", [
+    (1, 1, 1, 16, 4, 256), (1, 4, 4, 16, 4, 256), (3, 4, 9, 8, 2, 128), (24, 8, 192, 16, 4, 256), (64, 1, 64, 16, 4, 256),
+    (30, 2, 60, 32, 8, 128), (40, 8, 320, 16, 4, 256), (1, 64, 64, 16, 4, 256), (1, 512, 512, 16, 4, 256),
+    (12, 100, 1200, 4, 2, 128), (2, 9, 11, 24, 1, 128), (100, 30, 200, 4, 1, 128), (255, 2, 300, 16, 1, 256),
+    (1, 40, 40, 32, 8, 128), (5, 17, 80, 6, 6, 256),
+])
+def test_a_workspace_serves_every_call_of_fewer_keys(B, L, T, Hq, Hkv, D):
+    """The bytes of a call whose splits are chosen for it never fall as its keys grow, over every form it may take."""
+    f = _C.lib().qvex_paged_attention_workspace_bytes
+    keys = [*range(1, 6000, 37), *(128 * s + e for s in range(1, 400) for e in (0, 1)), *range(60000, 1 << 20, 40961)]
+    sizes = [f(B, L, T, Hq, Hkv, D, mk, 0) for mk in sorted(keys)]
+    assert sizes == sorted(sizes)

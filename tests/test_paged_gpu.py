@@ -568,3 +568,19 @@ def test_a_prompt_and_its_decode_steps(dev, fmt, D, Hq, n_kv):
     assert bool(((torch.cat(outs).cpu().double() - want).abs() <= tol).all())
     wq, wk, wv = ref.qk_rope(proj, w, w, Hq, n_kv, D, freqs.cpu(), 1e-6, torch.arange(T))
     assert bool(((q.double() - wq).abs() <= 2.0 ** -8 * wq.abs() + 2.0 ** -19 * wq.abs().amax(-1, keepdim=True)).all())
+
+
+@pytest.mark.parametrize("T,kps", [(1, 0), (4, 0), (4, 256), (40, 0)])
+def test_one_workspace_for_a_growing_context(dev, T, kps):
+    """A buffer made once for the longest context serves every shorter bound, with the bits of a buffer of the call's own."""
+    D, Hq, n_kv, page = 256, 16, 4, 64
+    pages = paged.KVPages.alloc(320, n_kv, D, "int8", page, dev)
+    table, pos = i32([list(range(320))], dev), i32([0], dev)
+    kv = torch.randn((20480, n_kv, D), generator=gen(60)).to(BF16).to(dev)
+    paged.kv_append(pages, kv, kv.flip(0), table, pos)
+    q = torch.randn((T, Hq, D), generator=gen(61)).to(BF16).to(dev)
+    ws = torch.empty(paged.workspace_bytes(pages, 1, T, Hq, 20000, keys_per_split=kps), dtype=torch.uint8, device=dev)
+    for keys in (20000, 16384, 9000, 8192, 3000, 300, T):
+        pos.fill_(keys - T)
+        a = paged.attention(pages, q, table, pos, keys, keys_per_split=kps, workspace=ws)
+        assert torch.equal(a, paged.attention(pages, q, table, pos, keys, keys_per_split=kps))
