@@ -273,7 +273,7 @@ def workspace_bytes(pages: KVPages, B: int, T: int, Hq: int, max_keys: int, max_
                     keys_per_split: int = 0) -> int:
     """Bytes of workspace that attention() takes for T rows of B sequences (0: none), with cu or
     without, at this max_keys or any smaller one. max_keys as there, at most the table's capacity."""
-    widths = {T, T // B} if max_rows is None else {max(1, min(int(max_rows), T))}
+    widths = {T if max_rows is None else max(1, min(int(max_rows), T)), T // B}
     return max(_workspace_bytes(B, L, T, Hq, pages.n_kv, pages.head_dim, int(max_keys), int(keys_per_split))
                for L in widths)
 

@@ -410,3 +410,12 @@ def test_a_workspace_serves_every_call_of_fewer_keys(B, L, T, Hq, Hkv, D):
     keys = [*range(1, 6000, 37), *(128 * s + e for s in range(1, 400) for e in (0, 1)), *range(60000, 1 << 20, 40961)]
     sizes = [f(B, L, T, Hq, Hkv, D, mk, 0) for mk in sorted(keys)]
     assert sizes == sorted(sizes)
+
+
+def test_workspace_bytes_with_max_rows_covers_calls_without_row_offsets():
+    """max_rows bounds a ragged call's rows only; without offsets every sequence has T / B."""
+    pages = paged.KVPages.alloc(64, 4, 256, "int8", 64, "cpu")
+    f = _C.lib().qvex_paged_attention_workspace_bytes
+    for B, T, rows in ((4, 64, 1), (2, 128, 4), (16, 16, 9), (8, 4, 2)):
+        got = paged.workspace_bytes(pages, B, T, 16, 4000, max_rows=rows)
+        assert got >= f(B, rows, T, 16, 4, 256, 4000, 0) and got >= f(B, max(T // B, 1), T, 16, 4, 256, 4000, 0)
