@@ -416,6 +416,6 @@ def test_workspace_bytes_with_max_rows_covers_calls_without_row_offsets():
     """max_rows bounds a ragged call's rows only; without offsets every sequence has T / B."""
     pages = paged.KVPages.alloc(64, 4, 256, "int8", 64, "cpu")
     f = _C.lib().qvex_paged_attention_workspace_bytes
-    for B, T, rows in ((4, 64, 1), (2, 128, 4), (16, 16, 9), (8, 4, 2)):
+    for B, T, rows in ((1, 16, 8), (2, 8, 9), (2, 32, 8), (2, 32, 64), (2, 128, 100), (8, 4, 2)):
         got = paged.workspace_bytes(pages, B, T, 16, 4000, max_rows=rows)
         assert got >= f(B, rows, T, 16, 4, 256, 4000, 0) and got >= f(B, max(T // B, 1), T, 16, 4, 256, 4000, 0)
