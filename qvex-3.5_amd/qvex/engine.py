@@ -17,7 +17,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from . import _C
+from . import _C, paged
 from .model import Qwen35
 from .mtp import MTPHead
 from .sampler import Sampler, SamplingParams
@@ -73,7 +73,8 @@ def generate(model: Qwen35, prompt_ids, params: SamplingParams, mtp: MTPHead | N
     (engine/engine.py:280-300). `forced` is shared with the
     generator: ids appended to it while iterating are emitted next, as the
     reference's reasoning budget does. A stop id counts in completion_tokens but
-    is not returned. kv: how keys and values are kept (Qwen35.make_cache). Stats keys
+    is not returned. kv: how keys and values are kept (Qwen35.make_cache); of a PagePool
+    the call holds what its prompt and max_tokens need while it runs. Stats keys
     follow the reference's (engine/engine.py:340-357) where they apply to this path."""
     use_mtp = mtp_policy(mtp_mode, mtp)
     ids = torch.as_tensor(prompt_ids, dtype=torch.int32).reshape(1, -1).to(model.norm.device)
@@ -88,7 +89,8 @@ def generate(model: Qwen35, prompt_ids, params: SamplingParams, mtp: MTPHead | N
     # the last one: the caches grow when they must (engine/model.py:156-170),
     # but sized up front the captured cycle is never captured again for room
     need = ids.shape[1] + limit + 2 * k + 2
-    cap = max(model.max_context, need)
+    # (pages of a pool that others use too: no more than that)
+    cap = need if isinstance(kv, paged.PagePool) else max(model.max_context, need)
     cache = model.make_cache(max_context=cap, kv=kv)
     mcache = mtp.make_cache(max_context=cap, kv=kv) if mtp is not None else None
     logits, last_h = prefill(model, ids, cache, mtp, mcache)

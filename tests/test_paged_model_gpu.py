@@ -205,3 +205,23 @@ def test_one_token_prompt_on_a_fresh_head(dev, fmt):
     on = generate(model, [17], params, random_mtp(model, seed=8), "on", kv=fmt)
     assert on.stats["mtp_graph_cycles"] == on.stats["mtp_cycles"] > 0
     assert on.tokens == generate(model, [17], params, None, "off", kv=fmt).tokens and len(on.tokens) == 12
+
+
+def test_generate_takes_what_it_needs_of_a_pool(dev, tiny):
+    """Pages for the prompt and max_tokens, not for the model's max_context: two sequences of one fixed pool at a
+    time (the second held by a cache), and a call that needs more raises with the pool as it was."""
+    model = random_model(Config.tiny(layers=4, vocab=2048), seed=5, device=dev, max_context=4096)
+    mtp = random_mtp(model, seed=6)
+    cfg = model.cfg
+    params = SamplingParams(temperature=0.0, top_k=0, top_p=1.0, max_tokens=20)
+    ids = ids_of(40, cfg.vocab_size, 6)
+    pool = paged.PagePool(12, cfg.num_key_value_heads, cfg.head_dim, "int8", 64, dev)
+    other = model.make_cache(max_context=200, kv=pool)              # 4 pages; the call: 4 for the layer, 4 for the head
+    got = generate(model, ids, params, mtp, "on", kv=pool)
+    assert got.tokens == generate(model, ids, params, mtp, "on", kv="int8").tokens and got.stats["mtp_graph_cycles"] > 0
+    assert got.tokens == generate(model, ids, params, mtp, "on", kv=pool, max_tokens=20).tokens
+    assert len(pool.free) == 8
+    with pytest.raises(_C.QvexError, match="free pages of 12"):
+        generate(model, ids, params, mtp, "on", kv=pool, max_tokens=300)
+    del other
+    assert len(pool.free) == 12
