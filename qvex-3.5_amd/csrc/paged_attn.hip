@@ -377,10 +377,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
 
 // A call of more than 8 rows per sequence takes the chunk form (paged_chunk.hip) if a sequence's
 // rows of a kv head fill half a block (a quarter on average, whatever L allows) and (query, key) pairs
-// * D are worth its start and end, 8 us against 3. us, this form | that one, int8, 16 query and 4 kv heads of 256 (pairs = T * Hq *
-// max_keys): 64 positions at 1000 keys (1.1M) 23 | 24, at 4000 (4.2M) 34 | 33, 512 at 0 (4.2M) 30 | 27,
-// 8 x 64 at 1000 (8.7M) 47 | 39, at 4000 (33M) 111 | 72, 512 at 4000 (37M) 119 | 75; of 128, 4 and 2
-// heads: 512 at 4000 (9.2M) 33 | 30, 12 x 100 at 1000 (5.3M) 24 | 24, 8 x 200 at 4000 (27M) 67 | 50.
+// * D are worth its start and end, 8 us against 3. us, this form | that one, 16 query and 4 kv heads of 256 (pairs = T * Hq *
+// max_keys), int8: 64 positions at 1000 keys (1.1M) 21 | 25, at 4000 (4.2M) 32 | 35, 512 at 0 (4.2M) 20 | 32,
+// 8 x 64 at 1000 (8.7M) 37 | 42, 64 at 8000 (8.3M) 44 | 40, 8 x 64 at 4000 (33M) 97 | 72, 512 at 4000 (37M) 100 | 75; bf16: 64 at
+// 4000 40 | 39, 8 x 64 at 1000 53 | 44, 512 at 4000 165 | 71; of 128, 4 and 2 heads, int8: 512 at 4000 (9.2M) 27 |
+// 29, 12 x 100 at 1000 (5.3M) 24 | 25, 8 x 200 at 4000 (27M) 62 | 49. One bound for all formats, between theirs.
 constexpr long PA_CHUNK_MIN = 64;
 // Many sequences of one tile and of long contexts are cut into equal runs of steps, one per CU (two of 128 dims), in
 // place of equal splits of each: a sequence far below max_keys leaves no CU idle, for a search in

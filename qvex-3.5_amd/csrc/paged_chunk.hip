@@ -10,20 +10,25 @@
 //   keys of one dim: V is stored in LDS by dims, its keys in that order.
 // LDS, in 16-byte units: K's row r holds unit c at c ^ (r % 16); V's row of dim d is
 // row d with its low two bits XORed by d / 16 % 4, unit c at c ^ (d / 4 % 4) ^ (d / 64): the 16
-// lanes of one pass of a read hit 16 different bank groups, and those of a write too.
+// lanes of one pass of a read hit 16 different bank groups. Writes do not always: V's 8-byte halves cost 258 cycles of
+// conflicts a step, codes of K (a lane's 16 are two units, so a pass hits every other unit of a row) 255.
 // A lane's 16 keys of a tile are one scale each for all its rows: a 16-lane row of
 // the wave holds them, and a product takes scale i by DPP broadcast.
-// Scores, m, l and O as in paged_attn.hip, but P is one bf16 term (2^-8 of a weight at
-// most, so 1.1e-3 of the output's norm beside the 1.7e-3 of its own rounding): the second
-// term would be a third product as long as the two.
+// Scores, m, l, O and the two bf16 terms of P as in paged_attn.hip: the output's error is its own rounding's (1.66e-3 of
+// its norm; with one term 2.34e-3). Both terms' products take one operand of V from LDS, and the terms are
+// made beside the products before, so the second costs the matrix cores' time (us, one term | two: after 16384 keys
+// int8 185 | 215, bf16 165 | 198, fp8 171 | 194, after 3584 bf16 61 | 69, merge included).
 //
-// 16 query and 4 kv heads of 256: 512 positions after 3584 bf16 keys 57 us and 8.6 of merging (500
-// TFLOP/s), after 16384 int8 keys 173 to 185 and 8.6 (760). One wave per SIMD holds 32 rows of Q and O in 192
-// registers, and what bounds it is its own issue: a step of 64 int8 keys has 64 products (2048 cycles) and some
-// 800 other instructions of 4 cycles, of which codes to bf16 and their way to LDS are 300. Two waves per SIMD that share 32 rows (each one key tile's scores, half the dims of O, weights
-// exchanged in LDS) measured us, int8 | bf16 after 16384 keys | bf16 after 3584: 171 | 168 | 65, this
-// 185 | 171 | 62 (merge included). A taken branch costs a lone wave some 200 cycles (rescaling O under a branch per
-// tile of it 294 us against 189), so what is rare lies behind the loop (fp8 187 -> 180).
+// 16 query and 4 kv heads of 256: 512 positions after 3584 bf16 keys 63 to 66 us and 8.8 of merging, after 16384
+// int8 keys 204 to 210 and 8.5 (670 TFLOP/s, the second term's products not counted). One wave per SIMD holds
+// 32 rows of Q and O in 192 registers. By the counters a step of 64 int8 keys takes 6,850 cycles: in 60 % of them the
+// wave issues (96 products, 700 other vector, 150 LDS instructions, 4 cycles each), in 19 % it waits for a matrix core
+// that is busy (44 % of the time), in 21 % for LDS (active 30 %), memory or the barrier. No one of them bounds it alone: what stands
+// beside no product, the scores' scales, maxima and vote, a lone wave cannot hide. Two waves per SIMD that share 32 rows (each one key
+// tile's scores, half the dims of O, weights exchanged in LDS) measured, with one term, us, int8 | bf16 after
+// 16384 keys | bf16 after 3584: 171 | 168 | 65 against 185 | 171 | 62 (merge included). A taken branch costs a lone
+// wave some 200 cycles (rescaling O under a branch per tile of it 294 us against 189), so what is rare lies behind the
+// loop (fp8 187 -> 180).
 #include "paged_attn.h"
 
 namespace {
@@ -55,6 +60,10 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
   constexpr int LPR = ROW / 16, KSTEP = 256 / LPR;   // lanes per key row, keys per load of the block
   constexpr int E = D / 16, VW = E * EB / 4;     // a thread's part of V and step: E dims (VW words) of four keys
   constexpr int K_BYTES = PC_KEYS * D * 2, STAGE = 2 * K_BYTES;
+  // the product of V that the next step's V starts beside: any, or (fewer products to spread it over) the second tile's
+  // (us after 16384 keys, the first | the second tile's: 256-dim heads int8 214 | 215, bf16 200 | 203, fp8 198 | 202,
+  // 128-dim heads 250 | 250, 217 | 217, 240 | 233)
+  constexpr int V_FIRST = D == 256 ? 0 : 2 * NT;
   __shared__ __align__(1024) uint8_t lds[2 * STAGE];
   __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -263,6 +272,12 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
       pc_f32x16 sc[2] = {zero, zero};
       u32x4 ring[PC_AHEAD];
       float wt[16];                                             // a tile's weights
+      u32x4 p[2], p_lo[2];                                      // and as two bf16 terms, 8 t .. + 7 of them
+      auto split = [&](int t, int e) __attribute__((always_inline)) {
+        const float w0 = wt[8 * t + 2 * e], w1 = wt[8 * t + 2 * e + 1];
+        p[t][e] = pa_pack(w0, w1);
+        p_lo[t][e] = pa_pack(w0 - bf16_lo(p[t][e]), w1 - bf16_hi(p[t][e]));
+      };
       // the scores of key tile kt, scaled and masked; m moved if they pass it (what has it as its reference follows)
       auto finish = [&](int kt) __attribute__((always_inline)) {
         if constexpr (EB == 1) scale16(sc[kt], ksc[kt]);
@@ -287,9 +302,12 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
             o[n] *= f;
             __builtin_amdgcn_sched_barrier(0);                  // a tile of O at a time
           }
-          if (kt == 1)
+          if (kt == 1) {
 #pragma unroll
             for (int x = 0; x < 16; ++x) wt[x] *= f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split(0, e);
+          }
         }
       };
       // weight x of tile kt, times its value's scale
@@ -300,13 +318,6 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         asm volatile("" : "+v"(w));                             // evaluated here, beside a product
         wt[x] = w;
       };
-      auto packed = [&](int t) __attribute__((always_inline)) {
-        u32x4 p;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = pa_pack(wt[8 * t + 2 * e], wt[8 * t + 2 * e + 1]);
-        return p;
-      };
-
 #pragma unroll
       for (int x = 0; x < PC_AHEAD; ++x) ring[x] = operand(x);
 #pragma unroll
@@ -326,33 +337,36 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         ring[x % PC_AHEAD] = operand(x + PC_AHEAD);
 #pragma unroll
         for (int y = st * 16 / KS; y < (st + 1) * 16 / KS; ++y) weight(0, y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)                             // halfway: the first eight are there
+          if (st == KS / 2 + e * (KS / 8)) split(0, e);
         __builtin_amdgcn_sched_barrier(0);
       }
       finish(1);
-      u32x4 p0 = packed(0), p1 = packed(1);
-#pragma unroll
-      for (int y = 0; y < 2 * NT; ++y) {
-        const int x = 2 * KS + y;
-        o[y % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_pa8(ring[x % PC_AHEAD]), as_pa8(y < NT ? p0 : p1), o[y % NT],
-                                                            0, 0, 0);
-        ring[x % PC_AHEAD] = operand(x + PC_AHEAD);
-#pragma unroll
-        for (int z = y * 8 / NT; z < (y + 1) * 8 / NT; ++z) weight(1, z);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      p0 = packed(0);
-      p1 = packed(1);
-      clean(kb + PC_KEYS, ok_next);
-#pragma unroll
-      for (int y = 0; y < 2 * NT; ++y) {                        // beside the next step's V
-        const int x = 2 * KS + 2 * NT + y;
-        o[y % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_pa8(ring[x % PC_AHEAD]), as_pa8(y < NT ? p0 : p1), o[y % NT],
-                                                            0, 0, 0);
+      if (V_FIRST == 0) clean(kb + PC_KEYS, ok_next);
+      // products y of V, two to an operand, beside the other tile's weights and the next step's V
+      auto add_v = [&](int y) __attribute__((always_inline)) {
+        const int x = 2 * KS + y, t = y / NT % 2;
+        const u32x4 v = ring[x % PC_AHEAD];
+        o[y % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_pa8(v), as_pa8(p[t]), o[y % NT], 0, 0, 0);
+        o[y % NT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_pa8(v), as_pa8(p_lo[t]), o[y % NT], 0, 0, 0);
         if (x + PC_AHEAD < 2 * KS + 4 * NT) ring[x % PC_AHEAD] = operand(x + PC_AHEAD);
 #pragma unroll
-        for (int z = y * VP / (2 * NT); z < (y + 1) * VP / (2 * NT); ++z) stage_v(to, z);
+        for (int e = 0; e < 4; ++e)                             // the eight weights of the next NT products
+          if (y < 3 * NT && y % NT == e * (NT / 4)) split(1 - t, e);
+        if (y < 2 * NT)
+#pragma unroll
+          for (int z = y * 8 / NT; z < (y + 1) * 8 / NT; ++z) weight(1, z);
+        if (y >= V_FIRST)
+#pragma unroll
+          for (int z = (y - V_FIRST) * VP / (4 * NT - V_FIRST); z < (y - V_FIRST + 1) * VP / (4 * NT - V_FIRST); ++z) stage_v(to, z);
         __builtin_amdgcn_sched_barrier(0);
-      }
+      };
+#pragma unroll
+      for (int y = 0; y < 2 * NT; ++y) add_v(y);
+      if (V_FIRST != 0) clean(kb + PC_KEYS, ok_next);
+#pragma unroll
+      for (int y = 2 * NT; y < 4 * NT; ++y) add_v(y);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         ksc[kt] = ks_next[kt];

@@ -584,3 +584,39 @@ def test_one_workspace_for_a_growing_context(dev, T, kps):
         pos.fill_(keys - T)
         a = paged.attention(pages, q, table, pos, keys, keys_per_split=kps, workspace=ws)
         assert torch.equal(a, paged.attention(pages, q, table, pos, keys, keys_per_split=kps))
+
+
+@pytest.fixture()
+def two_terms(monkeypatch):
+    """The reference's tolerance for weights of two bf16 terms, whatever the number of rows."""
+    plain = ref.attention
+    monkeypatch.setattr(ref, "attention", lambda *a, **kw: plain(*a, **{**kw, "terms": 2}))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D,Hq,n_kv,page,lens,pos,kps", [
+    (256, 16, 1, 256, [40], [300], 0), (128, 4, 2, 32, [130, 1, 65], [0, 200, 63], 0), (256, 4, 4, 64, [70], [0], 1 << 20),
+    (128, 4, 4, 16, [70, 0, 9], [5, 40, 127], 256), (256, 8, 4, 16, [33], [190], 1 << 20), (256, 16, 4, 64, [20], [0], 0),
+])
+def test_weights_keep_two_terms_in_calls_of_many_rows(dev, two_terms, fmt, wide, D, Hq, n_kv, page, lens, pos, kps):
+    """Both forms that serve more than 8 rows, of few rows and of prompt chunks (wide), hold a weight in 16 bits."""
+    check_attention(dev, fmt, D, Hq, n_kv, page, lens, pos, kps=kps, gate=kps == 0, wide=wide)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,Hq,n_kv", [(256, 8, 4), (128, 8, 2)])
+def test_prompt_chunk_whose_scores_rise(dev, two_terms, fmt, D, Hq, n_kv):
+    """Scores that grow along the keys move the reference in every step, between a tile's weights and their terms too."""
+    def edit(pool, q, tab):
+        q.fill_(0.0)
+        q[:, :, 0] = 1.0
+        for x in range(300):
+            j, s = pool.slot(tab[0], x)
+            k = pool.k[j, :, s].float() * 0.125
+            k[:, 0] = float(x if x % 7 else x - 40) * 4.0
+            v = pool.get((j, s))[1]
+            pool.put((j, s), k if fmt == "bf16" else k.clamp(-2000, 2000), v)
+
+    check_attention(dev, fmt, D, Hq, n_kv, 16, [100], [200], edit=edit, wide=True, scale=0.5)
+    check_attention(dev, fmt, D, Hq, n_kv, 16, [100], [200], edit=edit, wide=True, scale=0.5, kps=1 << 20, gate=True)
