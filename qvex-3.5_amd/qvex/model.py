@@ -1017,6 +1017,9 @@ class Qwen35:
         ids = torch.as_tensor(ids, device=self.norm.device).reshape(-1)
         L = ids.numel()
         counters = cache.counters
+        if not counters.graph_mode:
+            # every layer's pages before any layer runs: a pool that runs out leaves the caches as they were
+            paged.PagedKVCache.grow_all(cache, L)
         # chunk long inputs so every call fits the conv rings (prefill)
         step = L
         for c in cache:

@@ -390,9 +390,12 @@ class PagedKVCache:
     def state(self):
         return self.pages.tensors()
 
-    def _extend(self, min_capacity: int) -> None:
+    def _pages_for(self, min_capacity: int) -> int:
         size = -(-min_capacity // self.step) * self.step
-        self.ids += self.pool.take(-(-size // self.pool.page) - len(self.ids))
+        return -(-size // self.pool.page) - len(self.ids)
+
+    def _extend(self, min_capacity: int) -> None:
+        self.ids += self.pool.take(self._pages_for(min_capacity))
         self._upload()
 
     def _upload(self) -> None:
@@ -424,6 +427,25 @@ class PagedKVCache:
             return False
         self._extend(min_capacity)
         return True
+
+    @staticmethod
+    def grow_all(caches, extra: int) -> None:
+        """Pages for `extra` positions past the offset of every paged cache among `caches`, or, where a
+        pool cannot give them, an error with none of them changed."""
+        short = [c for c in caches if isinstance(c, PagedKVCache) and c.offset + extra > c.capacity]
+        for c in short:
+            c.counters._check_host_edit()
+        got = []
+        try:
+            for c in short:
+                got.append((c, c.pool.take(c._pages_for(c.offset + extra))))
+        except BaseException:
+            for c, ids in got:
+                c.pool.give(ids)
+            raise
+        for c, ids in got:
+            c.ids += ids
+            c._upload()
 
     def clone(self, counters=None) -> "PagedKVCache":
         """A cache of the same keys that shares the prefix's whole pages; counters:

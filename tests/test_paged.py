@@ -419,3 +419,30 @@ def test_workspace_bytes_with_max_rows_covers_calls_without_row_offsets():
     for B, T, rows in ((1, 16, 8), (2, 8, 9), (2, 32, 8), (2, 32, 64), (2, 128, 100), (8, 4, 2)):
         got = paged.workspace_bytes(pages, B, T, 16, 4000, max_rows=rows)
         assert got >= f(B, rows, T, 16, 4, 256, 4000, 0) and got >= f(B, max(T // B, 1), T, 16, 4, 256, 4000, 0)
+
+
+def test_caches_grow_together_or_not_at_all():
+    """Layers of one model: pages for all of them, or an error that leaves every cache and the pool as they were."""
+    from qvex.model import CacheCounters, KVCache
+    counters = CacheCounters(4, "cpu")
+    pool, other = (paged.PagePool(40, 2, 128, "int8", 16, "cpu") for _ in range(2))
+    dense = KVCache(counters, 3, n_kv=2, head_dim=64, capacity=256, device="cpu")
+    caches = [paged.PagedKVCache(other, counters, 0, capacity=1), paged.PagedKVCache(pool, counters, 1, capacity=1), dense,
+              paged.PagedKVCache(pool, counters, 2, capacity=1)]
+    for c in caches:
+        c.offset = 250
+    kv = [caches[0], caches[1], caches[3]]
+    before = [(list(c.ids), c.table.tolist()) for c in kv], list(pool.holders), list(other.holders)
+    with pytest.raises(_C.QvexError, match="free pages"):
+        paged.PagedKVCache.grow_all(caches, 7)           # 8 pages left in the pool, 16 and 16 more are needed
+    assert before == ([(list(c.ids), c.table.tolist()) for c in kv], list(pool.holders), list(other.holders))
+    paged.PagedKVCache.grow_all(caches, 6)               # they fit
+    assert before[0] == [(list(c.ids), c.table.tolist()) for c in kv]
+    pool.growable = True
+    paged.PagedKVCache.grow_all(caches, 7)
+    for c, (ids, _) in zip(kv, before[0]):
+        assert c.capacity == 512 and c.ids[:16] == ids and c.table[0].tolist() == c.ids and c.offset == 250
+    assert dense.capacity == 256
+    counters.graph_mode = True
+    with pytest.raises(_C.QvexError, match="captured cycle"):
+        paged.PagedKVCache.grow_all(caches, 300)

@@ -225,3 +225,25 @@ def test_generate_takes_what_it_needs_of_a_pool(dev, tiny):
         generate(model, ids, params, mtp, "on", kv=pool, max_tokens=300)
     del other
     assert len(pool.free) == 12
+
+
+@pytest.mark.parametrize("n", [7, 40, 600])
+def test_a_call_without_pages_leaves_every_layer_as_it_was(dev, n):
+    """A pool that runs out at the second attention layer: the first one, and the recurrent ones, have not moved, and
+    the call goes through once there are pages."""
+    model = random_model(Config.tiny(layers=8, vocab=2048), seed=9, device=dev, max_context=256)
+    cfg = model.cfg
+    page = 64
+    need = -(-(250 + n) // 256) * 256 // page - 4                   # more pages of each of the two layers
+    pool = paged.PagePool(8 + need, cfg.num_key_value_heads, cfg.head_dim, "int8", page, dev)
+    prompt, more = ids_of(250, cfg.vocab_size, 1), ids_of(n, cfg.vocab_size, 2)
+    cache = model.make_cache(max_context=256, kv=pool)
+    model(prompt, cache)
+    with pytest.raises(_C.QvexError, match="free pages"):
+        model(more, cache)
+    assert cache.counters.host.tolist() == [250] * 8
+    pool.growable = True
+    got = model(more, cache, last_only=False)
+    other = model.make_cache(max_context=1024, kv="int8")
+    model(prompt, other)
+    assert torch.equal(got, model(more, other, last_only=False))
