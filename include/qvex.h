@@ -655,7 +655,7 @@ int qvex_paged_read(const qvex_kv_pages* pages, const qvex_kv_rows* rows, void* 
 
 /* Causal GQA attention of the rows over their sequences' pages: row i of sequence
  * b sees positions 0 .. pos[b] + i, scores scaled by `scale` (>= 0), out
- * [T, Hq, D] bf16 (a row that sees nothing gets zeros; an infinity or a NaN among the
+ * [T, Hq, D] bf16 (a row that sees nothing gets zeros, whatever its gate; an infinity or a NaN among the
  * values leaves that dim of the rows that see it not finite, and no other row's). q:
  * row t, head h at q + t*q_token + h*q_head; gate (or NULL): alike, out times
  * sigmoid(gate). max_keys bounds pos[b] + rows of every

@@ -215,9 +215,10 @@ struct PaGate {
 #pragma unroll
     for (int i = 0; i < 4; ++i) g[i] = gp[i];
   }
-  __device__ __forceinline__ void store(const PaArgs& a, int t, int h, int d, int D, const float (&o)[4]) const {
+  // seen: the row sees a key (one that does not is zero whatever its gate holds)
+  __device__ __forceinline__ void store(const PaArgs& a, int t, int h, int d, int D, const float (&o)[4], bool seen) const {
     float f[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-    if (a.gate) {
+    if (a.gate && seen) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = 1.0f / (1.0f + expf(-bf16_to_f32(g[i])));
     }

@@ -336,7 +336,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PaArgs a) {
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] *= inv;
-        PaGate(a, tok, head, d).store(a, tok, head, d, D, acc);
+        PaGate(a, tok, head, d).store(a, tok, head, d, D, acc, ll != 0.0f);
       } else {
         const size_t rec = SHARES ? ((size_t)kh * (a.shares + a.B) + blockIdx.x / a.c.Hkv + b) * PA_ROWS + rr
                                   : ((size_t)tok * a.Hq + head) * a.nsplit + split;
@@ -493,7 +493,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PaArgs a) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] *= inv;
-      gate.store(a, tok, h, d, D, o);
+      gate.store(a, tok, h, d, D, o, l != 0.0f);
     }
     if constexpr (WIDE) __syncthreads();
   }

@@ -65,6 +65,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
   // 128-dim heads 250 | 250, 217 | 217, 240 | 233)
   constexpr int V_FIRST = D == 256 ? 0 : 2 * NT;
   __shared__ __align__(1024) uint8_t lds[2 * STAGE];
+  __shared__ uint32_t blank[4];                  // rows of each wave that see nothing
   __shared__ int odd;                            // some V has a NaN or an infinity that not all rows see
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int li = lane & 31, hf = lane >> 5;
@@ -384,6 +385,8 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
 
     // O through LDS, so that a row is written as consecutive bytes: 16-byte unit c of row r at c ^ (r % 16)
     l += __shfl_xor(l, 32, 64);
+    const uint64_t none = __ballot(l == 0.0f);
+    if (lane == 0) blank[wave] = (uint32_t)none;
     float* ob = reinterpret_cast<float*>(lds);
     const float inv = a.nsplit > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(256, 1) void paged_chunk_kernel(PaArgs a) {
         *reinterpret_cast<float4*>(a.ws + (((size_t)tok * a.Hq + head) * a.nsplit + split) * D + 4 * c) = v;
       } else {
         const float y[4] = {v.x, v.y, v.z, v.w};
-        PaGate(a, tok, head, 4 * c).store(a, tok, head, 4 * c, D, y);
+        PaGate(a, tok, head, 4 * c).store(a, tok, head, 4 * c, D, y, !(blank[rr >> 5] >> (rr & 31) & 1));
       }
     }
     __syncthreads();

@@ -620,3 +620,36 @@ def test_prompt_chunk_whose_scores_rise(dev, two_terms, fmt, D, Hq, n_kv):
 
     check_attention(dev, fmt, D, Hq, n_kv, 16, [100], [200], edit=edit, wide=True, scale=0.5)
     check_attention(dev, fmt, D, Hq, n_kv, 16, [100], [200], edit=edit, wide=True, scale=0.5, kps=1 << 20, gate=True)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n,B,width,kps", [
+    (1, 3, 4, 0), (6, 3, 4, 1 << 20), (6, 6, 20, 128), (80, 3, 3000, 1 << 20), (80, 3, 3000, 0), (1, 48, 300, 0), (3, 48, 300, 0),
+])
+def test_rows_that_see_nothing_are_zero_whatever_their_gate(dev, fmt, n, B, width, kps):
+    """Rows before position 0 and of sequences without pages: a gate that is NaN there changes no bit of any row, in
+    every form (one split, merged splits, chunks, runs of steps)."""
+    D, Hq, n_kv, page = 128, 4, 2, 16
+    held = [(-4, 9, 5)[b % 3] for b in range(B)]
+    need = [0 if b % 3 == 2 else -(-(p + n) // page) if p + n > 0 else 0 for b, p in enumerate(held)]
+    pages = paged.KVPages.alloc(max(1, sum(need)), n_kv, D, fmt, page, dev)
+    table = torch.full((B, width), -1, dtype=torch.int32)
+    at = 0
+    for b, m in enumerate(need):
+        table[b, :m] = torch.arange(at, at + m)
+        at += m
+    table = table.to(dev)
+    kv = torch.randn((B * page * 6, n_kv, D), generator=gen(70)).to(BF16).to(dev)
+    paged.kv_append(pages, kv, kv.flip(0), table, i32([0] * B, dev))
+    q = torch.randn((B * n, Hq, D), generator=gen(71)).to(BF16).to(dev)
+    gate = torch.randn((B * n, Hq, D), generator=gen(72)).to(BF16).to(dev)
+    blind = torch.tensor([b % 3 == 2 or p + i < 0 for b, p in enumerate(held) for i in range(n)], device=dev)
+    bad = gate.clone()
+    bad[blind] = math.nan
+    cu = i32([n * b for b in range(B + 1)], dev)
+    for rows in (None, cu):
+        kw = {"cu": rows, "max_rows": n} if rows is not None else {}
+        a = paged.attention(pages, q, table, i32(held, dev), gate=gate, keys_per_split=kps, **kw)
+        for _ in range(3):
+            got = paged.attention(pages, q, table, i32(held, dev), gate=bad, keys_per_split=kps, **kw)
+            assert torch.equal(a, got) and bool((got[blind] == 0).all()) and bool((got[~blind] != 0).any())
