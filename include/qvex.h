@@ -35,7 +35,7 @@ enum qvex_status {
 /* Message of the last failed call on this thread ("" if none). */
 const char* qvex_last_error(void);
 
-/* ABI version: bumped whenever a signature changes. */
+/* ABI version: bumped whenever a signature changes or entry points are added. */
 int qvex_abi_version(void);
 
 /* ------------------------------------------------------------------------

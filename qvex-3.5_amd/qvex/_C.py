@@ -97,10 +97,10 @@ SIGNATURES: dict[str, list] = {
     "qvex_paged_attention": [PAGES, ROWS, P, LNG, LNG, I, I, I, P, LNG, LNG, F, P, P, U64, P],
 }
 
-# qvex_abi_version() of the library these bindings match (8: the RoPE table of
+# qvex_abi_version() of the library these bindings match (9: the qvex_paged_* entry points; 8: the RoPE table of
 # qvex_attn_qk_rope; 7: the rows argument of qvex_cycle_finish_ex; 6: the done flag of qvex_cycle_finish_ex; 4: qvex_mtp_input, qvex_embed_rms_parts, the deferred
 # reduction of qvex_qmv_w4g64_packed_argmax)
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _lib: ctypes.CDLL | None = None
 

@@ -201,3 +201,17 @@ def test_dequant_argument_rules():
         _C.call("qvex_w4g64_dequant", p, None, p, 4, 64, p, None)
     with pytest.raises(_C.QvexError, match="16-byte"):
         _C.call("qvex_w4g64_dequant", p, p, p, 4, 64, p + 2, None)
+
+
+def test_a_library_without_the_paged_entry_points_is_refused_by_its_version(tmp_path, monkeypatch):
+    """One of version 8, which had none of them: the version says so, not a missing symbol."""
+    import subprocess
+    src, so = tmp_path / "old.c", tmp_path / "old.so"
+    src.write_text('const char* qvex_last_error(void) { return ""; }\nint qvex_abi_version(void) { return 8; }\n'
+                   + "".join(f"int {n}(void) {{ return 0; }}\n" for n in _C.exported_symbols()
+                             if "paged" not in n and n not in ("qvex_last_error", "qvex_abi_version")))
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)], check=True)
+    monkeypatch.setattr(_C, "_lib", None)
+    monkeypatch.setattr(_C, "LIB_PATH", so)
+    with pytest.raises(_C.QvexError, match="ABI version 8"):
+        _C.lib()
