@@ -653,3 +653,75 @@ def test_rows_that_see_nothing_are_zero_whatever_their_gate(dev, fmt, n, B, widt
         for _ in range(3):
             got = paged.attention(pages, q, table, i32(held, dev), gate=bad, keys_per_split=kps, **kw)
             assert torch.equal(a, got) and bool((got[blind] == 0).all()) and bool((got[~blind] != 0).any())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_graph_after_its_table_was_rewritten(dev, fmt):
+    """A captured step replayed after every sequence has moved to other pages, twice, beside the eager step."""
+    D, Hq, n_kv, page, B, W = 128, 4, 2, 16, 3, 12
+    pages = paged.KVPages.alloc(2 * B * W, n_kv, D, fmt, page, dev)
+    perm = torch.randperm(2 * B * W, generator=gen(80)).to(torch.int32)
+    table = perm[:B * W].view(B, W).to(dev)
+    pos = i32([0] * B, dev)
+    held = [100, 17, 150]
+    kv = torch.randn((B, 200, n_kv, D), generator=gen(81)).to(BF16).to(dev)
+    rows, cu = torch.cat([kv[b, :n] for b, n in enumerate(held)]), i32(offsets(held), dev)
+    k, q = torch.empty((B, n_kv, D), dtype=BF16, device=dev), torch.empty((B, Hq, D), dtype=BF16, device=dev)
+
+    def step():
+        paged.kv_append(pages, k, k, table, pos)
+        return paged.attention(pages, q, table, pos), *paged.kv_read(pages, table, pos, B)
+
+    def fill():
+        pos.zero_()
+        paged.kv_append(pages, rows, rows.flip(0), table, pos, cu)
+        pos.copy_(i32(held, dev))
+
+    k.zero_()
+    q.zero_()
+    fill()
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step()
+    for i in range(4):
+        old = table.clone()
+        at = torch.arange(B * W) + (0, B * W, 5, 31)[i]
+        table.copy_(perm[at % (2 * B * W)].view(B, W).roll(i, 0))
+        assert i == 0 or not bool((table == old).any())
+        for x in pages.tensors():
+            x.view(torch.uint8).zero_()
+        fill()
+        for j in range(2):
+            k.copy_(kv[:, 180 + i + j])
+            q.copy_(torch.randn((B, Hq, D), generator=gen(82 + 2 * i + j)).to(BF16))
+            for o in outs:
+                o.fill_(3.0)
+            g.replay()
+            torch.cuda.synchronize()
+            want = step()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+            assert bool((outs[0] != 0).all()) and bool((outs[1] != 0).any())
+            pos += 1
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_rows_keep_their_bits_in_large_ragged_calls_of_up_to_8(dev, fmt):
+    """With max_rows given, sequences of up to 8 rows in a call large enough for the chunk form, against calls of their own."""
+    D, Hq, n_kv, page, B, n = 128, 8, 2, 16, 20, 700
+    pages = paged.KVPages.alloc(B * 50, n_kv, D, fmt, page, dev)
+    table = torch.randperm(B * 50, generator=gen(90)).to(torch.int32).view(B, 50).to(dev)
+    kv = torch.randn((B * 750, n_kv, D), generator=gen(91)).to(BF16).to(dev)
+    paged.kv_append(pages, kv, kv.flip(0), table, i32([0] * B, dev))
+    lens = [8 if b % 4 else 1 + b % 7 for b in range(B)]
+    pos = i32([n - 13 * b for b in range(B)], dev)
+    cu, T = offsets(lens), sum(lens)
+    q = torch.randn((T, Hq, D), generator=gen(92)).to(BF16).to(dev)
+    wide = torch.cat([table, torch.full((B, 1000), -1, dtype=torch.int32, device=dev)], 1)
+    assert T * Hq * 1050 * page * D > 1.28e9
+    whole = paged.attention(pages, q, wide, pos, cu=i32(cu, dev), max_rows=8, keys_per_split=256)
+    for b in range(B):
+        for i in (0, lens[b] - 1):
+            one = paged.attention(pages, q[cu[b] + i:cu[b] + i + 1], table[b:b + 1], pos[b:b + 1] + i, keys_per_split=256)
+            assert torch.equal(one[0], whole[cu[b] + i])
