@@ -659,10 +659,10 @@ int qvex_paged_read(const qvex_kv_pages* pages, const qvex_kv_rows* rows, void* 
  * values leaves that dim of the rows that see it not finite, and no other row's). q:
  * row t, head h at q + t*q_token + h*q_head; gate (or NULL): alike, out times
  * sigmoid(gate). max_keys bounds pos[b] + rows of every
- * sequence (a larger one is still right, only slower). keys_per_split: keys per
+ * sequence (a longer one is still right, only slower). keys_per_split: keys per
  * block of a row's split (a multiple of 128), or 0 to choose by the call's size;
  * at one positive value a row's bits do not depend on the other rows of the call,
- * as long as the calls have up to 8 rows per sequence.
+ * as long as the calls have an L of up to 8.
  * workspace: qvex_paged_attention_workspace_bytes() of the same arguments, or of
  * a larger max_keys, 16-byte aligned (NULL where that is 0); it need not be cleared. */
 uint64_t qvex_paged_attention_workspace_bytes(int B, int L, int T, int Hq, int Hkv, int D,

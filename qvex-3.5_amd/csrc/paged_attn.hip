@@ -18,9 +18,9 @@
 // as two bf16 terms (16 bits of it), so the output's own rounding is the one that shows.
 //
 // 16 query and 4 kv heads of 256, int8: 64 sequences of one row at up to 8192 keys read 618 MB in 130 to 136 us
-// with a block per sequence and head (the CUs of the longest end last), in 120 and 6 of merging in equal runs (4.9
-// TB/s; a plain read reaches 6.2). One row at 4096 keys 6 us and 3.6 of merging, four at 7001 (fp8) 10 and
-// 4: two round trips of memory and two launches.
+// with a block per sequence and head (the CUs of the longest end last), in 117 and 6 of merging in equal runs (5.0
+// TB/s; a plain read reaches 6.2). One row at 4096 keys 6.8 us and 3.3 to 4.4 of merging, four at 7001 (fp8) 11 and
+// 3.5: two round trips of memory and two launches, on 132 and 112 blocks of 256 CUs and 16 and 64 of the merge.
 #include "paged_attn.h"
 
 namespace {
@@ -594,7 +594,9 @@ uint64_t pa_most_bytes(int B, int L, int T, int Hq, int Hkv, int D, int max_keys
 
 template <int FMT, int D>
 void launch_attn(dim3 grid, hipStream_t st, const PaArgs& a) {
-  constexpr bool FITS = FMT != QVEX_KV_BF16 || D == 128;         // 16 KB of K and of V per wave leave no registers over
+  // 16 KB of K and of V per wave leave no registers over: bf16 of 256 dims spills 6 registers without the prefetch, fp8 3
+  // with it, around the loop of steps (two of bf16's accesses are in it under SHARES)
+  constexpr bool FITS = FMT != QVEX_KV_BF16 || D == 128;
   // many rows: other tiles' waves hide the loads, and fewer registers are worth more (us, two rows' tiles or more, with |
   // without: 12 x 200 rows at 1500 keys 27.9 | 26.8; 2 x 64 at 1000 25.0 | 23.6; 16 x 12 at 2000 39.4 | 38.3)
   if (a.shares) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, FITS, true>), grid, dim3(256), 0, st, a);

@@ -943,7 +943,8 @@ class Qwen35:
                    kv: str | paged.PagePool | None = None):
         """One cache per layer. kv: how the attention layers keep keys and values - None:
         dense bf16 (KVCache); "bf16", "int8" or "fp8": in pages of that format
-        (PagedKVCache), from a pool of their own; a PagePool: in that pool's pages."""
+        (PagedKVCache), from a pool of their own of the capacity's pages, moved to larger
+        tensors when they run out; a PagePool: in that pool's pages."""
         cfg = self.cfg
         dev = self.norm.device
         cap = max_context or self.max_context

@@ -232,7 +232,8 @@ def attention(pages: KVPages, q: torch.Tensor, table: torch.Tensor, pos: torch.T
     their sequences' pages: row i of sequence b sees positions 0 .. pos[b] + i (append
     the rows' own keys first). gate [T, Hq, D]: the output times sigmoid(gate)
     (engine/model.py:228-232). scale: 1 / sqrt(D) if None. max_keys: a bound of pos[b] +
-    rows, the table's capacity if None. keys_per_split: see qvex_paged_attention.
+    rows, the table's capacity if None. keys_per_split: see qvex_paged_attention; the
+    promise on a row's bits takes max_rows of 8 or less where cu is given.
     workspace: any tensor of at least workspace_bytes(); one is made per call if None.
     Returns bf16 [T, Hq, D]; rows outside every sequence are left as they are in out."""
     T, Hq, qt, qh = pages._heads(q, "q")
@@ -342,8 +343,10 @@ class PagePool:
 class PagedKVCache:
     """One sequence's keys and values of one layer in a pool's pages, with KVCache's
     interface (offset, rollback, grow, clone, keys, values; engine/model.py:149-176).
-    Growing adds pages to its table and moves no key; a clone shares the whole
-    pages of the prefix and copies the one that the next key goes to.
+    Growing adds free pages of the pool to its table and moves no key (a growable pool
+    that has none left moves as a whole); a clone shares the whole pages of the prefix and
+    copies the one that the next key goes to. What finds too few pages raises, with
+    nothing changed.
 
     The page of position ``offset`` and all behind it have this cache as their only holder
     (clone and rollback see to it), so an append never writes a shared page."""
