@@ -432,9 +432,9 @@ class PagedKVCache:
         return True
 
     @staticmethod
-    def grow_all(caches, extra: int) -> None:
+    def grow_all(caches, extra: int) -> bool:
         """Pages for `extra` positions past the offset of every paged cache among `caches`, or, where a
-        pool cannot give them, an error with none of them changed."""
+        pool cannot give them, an error with none of them changed. Returns whether any grew."""
         short = [c for c in caches if isinstance(c, PagedKVCache) and c.offset + extra > c.capacity]
         for c in short:
             c.counters._check_host_edit()
@@ -449,6 +449,7 @@ class PagedKVCache:
         for c, ids in got:
             c.ids += ids
             c._upload()
+        return bool(got)
 
     def clone(self, counters=None) -> "PagedKVCache":
         """A cache of the same keys that shares the prefix's whole pages; counters:

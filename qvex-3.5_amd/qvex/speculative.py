@@ -22,6 +22,7 @@ from . import _C
 from .kernels import _ptr, _stream
 from .model import Qwen35, rope_table
 from .mtp import MTPHead
+from .paged import PagedKVCache
 from .sampler import Sampler
 
 MAX_PENDING = 1024
@@ -161,11 +162,22 @@ class MTPDecoder:
 GRAPH_GROW_MIN = 2048
 
 
-def grow_kv(caches, extra: int) -> bool:
+def grow_kv(caches, extra: int, least: int | None = None) -> bool:
     """Grow every KV cache among `caches` to hold `extra` positions past its
-    offset (KVCache.grow); returns whether any moved."""
-    moved = False
+    offset (KVCache.grow); returns whether any moved. Paged caches grow together; where
+    their pool has not so many pages, by less, down to `least` positions."""
+    extra_paged, least = extra, extra if least is None else least
+    while True:
+        try:
+            moved = PagedKVCache.grow_all(caches, extra_paged)
+            break
+        except _C.QvexError:
+            if extra_paged <= least:
+                raise
+            extra_paged = max(extra_paged // 4, least)
     for c in caches:
+        if isinstance(c, PagedKVCache):
+            continue
         if hasattr(c, "grow"):
             moved |= c.grow(c.offset + extra)
     return moved
@@ -188,8 +200,8 @@ def decode(model: Qwen35, sampler: Sampler, cache, first_logits, last_hidden=Non
     graph (the caches go back to eager control), and the next MTP cycle
     captures it again (10-30 ms), after one eager cycle when more than k + 1
     (hidden, token) pairs are pending. When the next cycle would not fit a KV
-    cache, the caches grow (by GRAPH_GROW_MIN positions or half their capacity)
-    and the cycle is captured on the new buffers. The token stream is the one
+    cache, the caches grow (by GRAPH_GROW_MIN positions or half their capacity, or by
+    what a page pool still has) and the cycle is captured on the new buffers. The token stream is the one
     graph=False (every cycle launched op by op from the host) emits."""
     forced = forced if forced is not None else []
     dec = MTPDecoder(model, sampler, cache, first_logits, last_hidden, mtp, mtp_cache, k, stats)
@@ -212,7 +224,7 @@ def decode(model: Qwen35, sampler: Sampler, cache, first_logits, last_hidden=Non
                     if g.room() < 1:
                         g.release()
                         kv = [c for c in dec.cache if hasattr(c, "grow")] + [dec.mtp_cache]
-                        grow_kv(kv, max(GRAPH_GROW_MIN, max(c.capacity for c in kv) // 2))
+                        grow_kv(kv, max(GRAPH_GROW_MIN, max(c.capacity for c in kv) // 2), 4 * (k + 1))
                         g.attach()
                         st["captures"] += 1
                     emitted = g.cycle()

@@ -446,3 +446,26 @@ def test_caches_grow_together_or_not_at_all():
     counters.graph_mode = True
     with pytest.raises(_C.QvexError, match="captured cycle"):
         paged.PagedKVCache.grow_all(caches, 300)
+
+
+def test_caches_of_a_small_pool_grow_by_what_it_has():
+    """Before a captured cycle: by the positions asked for, by less where the pool has less, and an error below `least`."""
+    from qvex.model import KVCache
+    from qvex.speculative import grow_kv
+    pool = paged.PagePool(112, 2, 128, "int8", 16, "cpu")
+    caches = [paged.PagedKVCache(pool, capacity=256) for _ in range(2)]
+    dense = KVCache(None, 0, n_kv=2, head_dim=64, capacity=256, device="cpu")
+    for c in (*caches, dense):
+        c.offset = 250
+    with pytest.raises(_C.QvexError, match="free pages"):
+        grow_kv([*caches, dense], 2048)
+    assert [c.capacity for c in (*caches, dense)] == [256, 256, 256]
+    assert grow_kv([*caches, dense], 2048, 16)                 # 80 pages: 512 positions for each, then
+    assert [c.capacity for c in (*caches, dense)] == [768, 768, 2304]
+    assert not grow_kv(caches, 100, 16)
+    for c in caches:
+        c.offset = 760
+    with pytest.raises(_C.QvexError, match="free pages"):
+        grow_kv(caches, 2048, 16)                              # 16 pages are left, 32 are needed
+    assert [c.capacity for c in caches] == [768, 768] and len(pool.free) == 16
+    assert grow_kv(caches[:1], 2048, 16) and [c.capacity for c in caches] == [1024, 768] and not pool.free

@@ -247,3 +247,19 @@ def test_a_call_without_pages_leaves_every_layer_as_it_was(dev, n):
     other = model.make_cache(max_context=1024, kv="int8")
     model(prompt, other)
     assert torch.equal(got, model(more, other, last_only=False))
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_decode_grows_by_what_a_small_pool_has(dev, tiny, graph):
+    """A fixed pool that two caches outgrow by 256 positions each: the captured cycle's larger steps are not taken, its
+    tokens are those of a pool of its own; past the last page the error leaves the caches with their keys."""
+    model, mtp = tiny
+    cfg = model.cfg
+    ids = ids_of(240, cfg.vocab_size, 7)
+    want, _, _ = run(model, mtp, ids, "int8", 60, cap=1024)
+    pool = paged.PagePool(16, cfg.num_key_value_heads, cfg.head_dim, "int8", 64, dev)
+    got, st, cache = run(model, mtp, ids, pool, 60, graph=graph, cap=256)
+    assert got == want and cache[-1].capacity == 512 and not cache.counters.graph_mode
+    assert not graph or st["graph_cycles"] > 0
+    with pytest.raises(_C.QvexError, match="free pages"):
+        run(model, mtp, ids, pool, 300, graph=graph, cap=256)
