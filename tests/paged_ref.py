@@ -95,8 +95,8 @@ def attention(pool, q, table, pos, cu=None, gate=None, scale=None, fill=0.0, ter
     of magnitudes, times 3 for its scale, its conversion to base 2 and the argument's
     subtraction), which moves its weight by as much, relatively, and the sum of
     the weights too; exp2 is good to 2 u; a weight goes into the product as two bf16 terms
-    (2^-16 of it), or, in calls of more than 8 rows per sequence (terms=1), as one (2^-8
-    of it); sums over n weights n u. The output is rounded to bf16 (2^-8)."""
+    (2^-16 of it; terms=1 is a looser bound, of a weight in one term, 2^-8 of it);
+    sums over n weights n u. The output is rounded to bf16 (2^-8)."""
     T, Hq, D = q.shape
     scale = D ** -0.5 if scale is None else scale
     out = torch.full((T, Hq, D), fill, dtype=torch.float64)
